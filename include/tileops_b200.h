@@ -295,6 +295,33 @@ TO_API int to_w8a8_fp8_gemm(const void* a, const void* b, const float* a_s, cons
  * aligned; other shapes, alignments and fp32 on 64 x 64 SIMT tiles. */
 TO_API int to_gemm(const void* a, const void* b, void* c, int dtype, int64_t M, int64_t N,
                    int64_t K, void* stream);
+/* Library extension (no reference counterpart): C = act(A @ B + bias) + residual in one kernel;
+ * A [M,K] rows lda apart, B [K,N] dense, bias [N] or NULL, residual [M,N] rows ldr apart or NULL,
+ * C [M,N] rows ldc apart, all of dtype F32, F16 or BF16; act one of TO_EPI_*. fp32 up to the one
+ * rounding of C. C may be the residual; it must not overlap A or B. Any M, N, K (K = 0: the
+ * epilogue of zeros). 16-bit operands run on tcgen05 tiles at any alignment, fp32 on SIMT tiles. */
+#define TO_EPI_NONE 0
+#define TO_EPI_RELU 1
+#define TO_EPI_SILU 2
+#define TO_EPI_GELU 3 /* tanh form */
+TO_API int to_gemm_bias_act(const void* a, int64_t lda, const void* b, const void* bias, int act,
+                            const void* residual, int64_t ldr, void* c, int64_t ldc, int dtype,
+                            int64_t M, int64_t N, int64_t K, void* stream);
+/* Library extension: the W8A8 products with the same epilogue, C = act(sum_kb (A_kb B_kb^T)[m,n]
+ * a_s[m,kb] b_s[n/block_n,kb] + bias) + residual. Operands and scales as to_w8a8_i8_gemm /
+ * to_w8a8_fp8_gemm; bias, residual and C of c_dtype. One rounding (to_w8a8_*_gemm with a bias
+ * rounds twice, as the reference does). block_k >= K or a multiple of 128 runs on tcgen05 tiles,
+ * any other block_k on SIMT tiles. */
+TO_API int to_w8a8_i8_gemm_bias_act(const int8_t* a, const int8_t* b, const float* a_s,
+                                    const float* b_s, const void* bias, int act,
+                                    const void* residual, int64_t ldr, void* c, int64_t ldc,
+                                    int c_dtype, int64_t M, int64_t N, int64_t K, int64_t block_n,
+                                    int64_t block_k, void* stream);
+TO_API int to_w8a8_fp8_gemm_bias_act(const void* a, const void* b, const float* a_s,
+                                     const float* b_s, const void* bias, int act,
+                                     const void* residual, int64_t ldr, void* c, int64_t ldc,
+                                     int c_dtype, int64_t M, int64_t N, int64_t K, int64_t block_n,
+                                     int64_t block_k, void* stream);
 /* replaces tileops/blas/gemv.py:22 gemv (and its mv alias, :60): y [M] = A [M,K] @ x [K], A
  * row-major, dtype F32, F16 or BF16 for A, x and y, fp32 accumulation, y rounded once. Any M, K
  * (K = 0 writes zeros); 16-byte loads when K * sizeof(dtype) % 16 == 0 and A, x are 16-byte
@@ -325,6 +352,20 @@ TO_API int to_act_and_mul_group_quant(const void* a, const void* b, int dtype, i
                                       int64_t cols, int64_t lda, int64_t ldb, int act,
                                       int64_t group_size, float eps, int ue8m0, int column_major,
                                       int q_dtype, void* q, float* scales, void* stream);
+/* Library extension (no reference counterpart): residual add, root-mean-square norm and per-group
+ * quantisation of [rows, cols] in one pass: h = x + residual (residual may be NULL), y = h /
+ * sqrt(mean(h^2) + eps) * weight, scale = max(max|y|, quant_eps) / qmax per group of group_size
+ * columns (group_size divides cols; q_dtype TO_E4M3: qmax 448, ue8m0 and column_major as
+ * to_per_token_group_quant_fp8; TO_I8: 127), q [rows, cols] the codes of y / scale, dense. fp32
+ * throughout; y is not rounded to dtype. h rounded to dtype goes to residual_out unless NULL
+ * (x or residual itself allowed). x, residual, residual_out rows ldx, ldr, ldh apart; weight
+ * [cols]; all four of dtype F32, F16 or BF16. */
+TO_API int to_add_rms_norm_group_quant(const void* x, int64_t ldx, const void* residual,
+                                       int64_t ldr, const void* weight, int dtype, int64_t rows,
+                                       int64_t cols, int64_t group_size, float eps,
+                                       float quant_eps, int ue8m0, int column_major, int q_dtype,
+                                       void* q, float* scales, void* residual_out, int64_t ldh,
+                                       void* stream);
 
 #ifdef __cplusplus
 }

@@ -36,6 +36,7 @@ from .quant_fp8 import (
     per_token_group_quant_fp8,
     per_token_group_quant_fp8_tma_aligned,
     w8a8_block_fp8_matmul,
+    w8a8_block_fp8_matmul_bias_act,
     w8a8_triton_block_scaled_mm,
 )
 from .quant_int8 import (
@@ -45,11 +46,17 @@ from .quant_int8 import (
     per_token_group_quant_int8,
     per_token_quant_int8,
     w8a8_block_int8_matmul,
+    w8a8_block_int8_matmul_bias_act,
     w8a8_int8_accumulators,
 )
 from ._lib import set_launch_overlap, version
-from .blas import gemm, gemv, mm, mv
-from .fused import act_and_mul_group_quant, gelu_and_mul, silu_and_mul
+from .blas import gemm, gemm_bias_act, gemv, mm, mv
+from .fused import (
+    act_and_mul_group_quant,
+    add_rms_norm_group_quant,
+    gelu_and_mul,
+    silu_and_mul,
+)
 
 __all__ = [
     "set_launch_overlap",
@@ -69,7 +76,9 @@ __all__ = [
     "block_dequant",
     "block_dequant_fp8",
     "w8a8_block_int8_matmul",
+    "w8a8_block_int8_matmul_bias_act",
     "w8a8_block_fp8_matmul",
+    "w8a8_block_fp8_matmul_bias_act",
     "w8a8_triton_block_scaled_mm",
     "w8a8_int8_accumulators",
     "apply_w8a8_block_int8_linear",
@@ -79,6 +88,7 @@ __all__ = [
     "awq_dequantize",
     "awq_dequantize_triton",
     "act_and_mul_group_quant",
+    "add_rms_norm_group_quant",
     "awq_gemm",
     "awq_gemm_gelu_and_mul",
     "awq_gemm_silu_and_mul",
@@ -90,6 +100,7 @@ __all__ = [
     "silu_and_mul",
     "gelu_and_mul",
     "gemm",
+    "gemm_bias_act",
     "mm",
     "gemv",
     "mv",

@@ -78,6 +78,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                     _L, _I, _P, _S, _P]),
     "to_act_and_mul_group_quant": (_I, [_P, _P, _I, _L, _L, _L, _L, _I, _L, _F, _I, _I, _I, _P,
                                         _P, _P]),
+    "to_add_rms_norm_group_quant": (_I, [_P, _L, _P, _L, _P, _I, _L, _L, _L, _F, _F, _I, _I, _I, _P,
+                                         _P, _P, _L, _P]),
     "to_peer_flags_bytes": (_S, []),
     "to_peer_barrier": (_I, [ctypes.POINTER(_P), _I, _I, _P, _P]),
     "to_ipc_alloc": (_I, [_S, ctypes.POINTER(_P), _P]),
@@ -87,6 +89,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "to_w8a8_i8_gemm": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _L, _L, _L, _L, _L, _P]),
     "to_w8a8_fp8_gemm": (_I, [_P, _P, _P, _P, _P, _I, _P, _L, _L, _L, _L, _L, _P]),
     "to_gemm": (_I, [_P, _P, _P, _I, _L, _L, _L, _P]),
+    "to_gemm_bias_act": (_I, [_P, _L, _P, _P, _I, _P, _L, _P, _L, _I, _L, _L, _L, _P]),
+    "to_w8a8_i8_gemm_bias_act": (_I, [_P, _P, _P, _P, _P, _I, _P, _L, _P, _L, _I, _L, _L, _L, _L,
+                                      _L, _P]),
+    "to_w8a8_fp8_gemm_bias_act": (_I, [_P, _P, _P, _P, _P, _I, _P, _L, _P, _L, _I, _L, _L, _L, _L,
+                                       _L, _P]),
     "to_gemv": (_I, [_P, _P, _P, _I, _L, _L, _P]),
     "to_silu_and_mul": (_I, [_P, _P, _P, _I, _L, _L, _L, _L, _L, _P]),
     "to_gelu_and_mul": (_I, [_P, _P, _P, _I, _L, _L, _L, _L, _L, _P]),

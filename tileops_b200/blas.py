@@ -7,6 +7,7 @@ This is the dense comparator of the quantized layers: the same tcgen05 tiles as 
 (kind::f16, A K-major, B read MN-major as 64-column strips, no scales). float16 and bfloat16
 run on those tiles when K % 8 == 0 and N % 64 == 0 with 16-byte aligned operands; other
 shapes, and float32, run on the library's SIMT tiles (fp32 FMA).
+``gemm_bias_act`` is the product with bias, activation and residual in its epilogue.
 GEMV runs on its own streaming kernel for float32, float16 and bfloat16 at every shape.
 """
 
@@ -16,7 +17,8 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from . import _epilogue, _lib
+from .fused import _row_stride
 
 
 def gemm(a: torch.Tensor, b: torch.Tensor, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -50,6 +52,44 @@ def gemm(a: torch.Tensor, b: torch.Tensor, *, out: Optional[torch.Tensor] = None
     if cc.data_ptr() != out.data_ptr():
         out.copy_(cc)
     return out
+
+
+def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                  act: Optional[str] = None, residual: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Library extension (no reference counterpart): ``C = act(A @ B + bias) + residual`` in one
+    kernel, A (M, K), B (K, N), bias (N,), residual (M, N), all of one dtype (float32, float16 or
+    bfloat16); ``act`` None, ``"relu"``, ``"silu"`` or ``"gelu"`` (tanh form, as in gelu_and_mul).
+    The sum, the bias, the activation and the residual are fp32 and C is rounded once. Rows of A,
+    residual and out may be strided. ``out`` may be ``residual`` (added in place); it must not
+    overlap A or B."""
+    op = "gemm_bias_act"
+    if a.ndim != 2 or b.ndim != 2:
+        raise ValueError(f"{op} expects 2-D A and B")
+    m, k = a.shape
+    k2, n = b.shape
+    if k != k2:
+        raise ValueError(f"{op}: incompatible shapes {tuple(a.shape)} @ {tuple(b.shape)}")
+    if a.dtype != b.dtype:
+        raise TypeError(f"{op}: A and B dtypes must match")
+    dtype = a.dtype
+    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"Unsupported dtype {dtype}; expected one of torch.float32, "
+                         "torch.float16, torch.bfloat16")
+    device = a.device
+    code = _epilogue.check(op, (m, n), n, dtype, device, bias, act, residual, out)
+    idx = _lib.ensure_device(a, op)
+    _lib.same_device(op, a, b)
+    lda = _row_stride(a)
+    if lda is None:
+        a, lda = a.contiguous(), k
+    if not b.is_contiguous():
+        b = b.contiguous()
+    bias, residual, ldr, dst, ldc = _epilogue.prepare((m, n), n, dtype, device, bias, residual, out)
+    _lib.call("to_gemm_bias_act", a.data_ptr(), lda, b.data_ptr(), _lib.ptr(bias), code,
+              _lib.ptr(residual), ldr, dst.data_ptr(), ldc, _lib.DTYPE_CODES[dtype], m, n, k,
+              _lib.stream_ptr(idx))
+    return _epilogue.finish(dst, out)
 
 
 def mm(input: torch.Tensor, mat2: torch.Tensor, *,
@@ -101,4 +141,4 @@ def mv(input: torch.Tensor, vec: torch.Tensor, *,
     return gemv(input, vec, out=out)
 
 
-__all__ = ["gemm", "gemv", "mm", "mv"]
+__all__ = ["gemm", "gemm_bias_act", "gemv", "mm", "mv"]

@@ -7,7 +7,7 @@
 // exact in fp32), one k-block at a time, then scaled and accumulated in fp32. This is the
 // path for small or ragged shapes (the reference tests use M=6, N=10, K=24, block [4,8]);
 // the tcgen05 kernels take the large per-token / per-channel shapes.
-#include "common.cuh"
+#include "linear_epi.cuh"
 
 namespace tob {
 namespace {
@@ -23,11 +23,21 @@ __device__ __forceinline__ void store_out(void* c, int64_t idx, float v, const v
   reinterpret_cast<T*>(c)[idx] = r;
 }
 
-template <bool FP8, typename TC>
+// One output of the fused epilogue: T(act(acc + bias) + residual), one rounding.
+template <typename T>
+__device__ __forceinline__ void finish_epi(const LinEpi& ep, int m, int n, float acc) {
+  if (ep.bias != nullptr) acc += to_f32(reinterpret_cast<const T*>(ep.bias)[n]);
+  float v = epi_act<false>(acc, ep.act);
+  if (ep.res != nullptr) v += to_f32(reinterpret_cast<const T*>(ep.res)[(int64_t)m * ep.ldr + n]);
+  reinterpret_cast<T*>(ep.c)[(int64_t)m * ep.ldc + n] = from_f32<T>(v);
+}
+
+// EPI: the fused epilogue of linear_epi.cuh in place of the plain store (c, bias unused).
+template <bool FP8, typename TC, bool EPI = false>
 __global__ void __launch_bounds__(kThreads) k_w8a8_generic(
     const uint8_t* __restrict__ a, const uint8_t* __restrict__ b, const float* __restrict__ a_s,
     const float* __restrict__ b_s, void* __restrict__ c, const void* __restrict__ bias,
-    int32_t* __restrict__ acc_out, int M, int N, int K, int bn, int bk) {
+    int32_t* __restrict__ acc_out, int M, int N, int K, int bn, int bk, const LinEpi ep) {
   __shared__ __align__(16) uint8_t As[kTM][kTK + 4];
   __shared__ __align__(16) uint8_t Bs[kTN][kTK + 4];
   const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;  // 16 x 16 threads, 4 x 4 outputs each
@@ -100,9 +110,13 @@ __global__ void __launch_bounds__(kThreads) k_w8a8_generic(
     for (int j = 0; j < 4; ++j) {
       const int gn = n0 + tn + 16 * j;
       if (gn >= N) continue;
-      const int64_t idx = (int64_t)gm * N + gn;
-      store_out<TC>(c, idx, accf[i][j], bias, gn);
-      if (!FP8 && acc_out) acc_out[idx] = acci_total[i][j];
+      if constexpr (EPI) {
+        finish_epi<TC>(ep, gm, gn, accf[i][j]);
+      } else {
+        const int64_t idx = (int64_t)gm * N + gn;
+        store_out<TC>(c, idx, accf[i][j], bias, gn);
+        if (!FP8 && acc_out) acc_out[idx] = acci_total[i][j];
+      }
     }
   }
 }
@@ -111,11 +125,12 @@ __global__ void __launch_bounds__(kThreads) k_w8a8_generic(
 // rounded once) for the shapes the tcgen05 tiles do not take (N % 64, K % 8, unaligned rows,
 // fp32; tileops/blas/gemm.py:31). 64 x 64 output tiles, 16 x 16 threads of 4 x 4 outputs, K in
 // steps of 32 through shared memory; every product in fp32 with fmaf in increasing k.
-template <typename T>
+// EPI: A with rows lda apart and the fused epilogue of linear_epi.cuh (c unused).
+template <typename T, bool EPI = false>
 __global__ void __launch_bounds__(kThreads) k_gemm_dense_simt(const T* __restrict__ a,
                                                              const T* __restrict__ b,
                                                              T* __restrict__ c, int M, int N,
-                                                             int K) {
+                                                             int K, int64_t lda, const LinEpi ep) {
   __shared__ float As[kTK][kTM + 4];  // transposed: As[k][m]
   __shared__ float Bs[kTK][kTN + 4];  // Bs[k][n]
   const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
@@ -126,7 +141,7 @@ __global__ void __launch_bounds__(kThreads) k_gemm_dense_simt(const T* __restric
     for (int i = threadIdx.x; i < kTM * kTK; i += kThreads) {
       const int r = i / kTK, kk = i % kTK;  // A: consecutive threads along k of one row
       const int gm = m0 + r, gk = k0 + kk;
-      As[kk][r] = (gm < M && gk < K) ? to_f32(a[(int64_t)gm * K + gk]) : 0.f;
+      As[kk][r] = (gm < M && gk < K) ? to_f32(a[(int64_t)gm * lda + gk]) : 0.f;
     }
     for (int i = threadIdx.x; i < kTK * kTN; i += kThreads) {
       const int kk = i / kTN, cc = i % kTN;  // B: consecutive threads along n of one row
@@ -154,7 +169,9 @@ __global__ void __launch_bounds__(kThreads) k_gemm_dense_simt(const T* __restric
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int gn = n0 + tn + 16 * j;
-      if (gn < N) c[(int64_t)gm * N + gn] = from_f32<T>(acc[i][j]);
+      if (gn >= N) continue;
+      if constexpr (EPI) finish_epi<T>(ep, gm, gn, acc[i][j]);
+      else c[(int64_t)gm * N + gn] = from_f32<T>(acc[i][j]);
     }
   }
 }
@@ -169,7 +186,7 @@ int gemm_dense_simt_launch(const void* a, const void* b, void* c, int dtype, int
   if (grid.y > 65535) return fail(TO_EUNSUPPORTED, "gemm: M too large for the SIMT tiles");
   TOB_DISPATCH_FLOAT(dtype, T, {
     k_gemm_dense_simt<T><<<grid, kThreads, 0, st>>>((const T*)a, (const T*)b, (T*)c, (int)M,
-                                                     (int)N, (int)K);
+                                                     (int)N, (int)K, K, LinEpi{});
   });
   return check_launch("gemm (SIMT tiles)");
 }
@@ -184,13 +201,48 @@ int w8a8_generic_launch(bool fp8, const void* a, const void* b, const float* a_s
     if (fp8)
       k_w8a8_generic<true, TC><<<grid, kThreads, 0, st>>>(
           (const uint8_t*)a, (const uint8_t*)b, a_s, b_s, c, bias, nullptr, (int)M, (int)N,
-          (int)K, (int)bn, (int)bk);
+          (int)K, (int)bn, (int)bk, LinEpi{});
     else
       k_w8a8_generic<false, TC><<<grid, kThreads, 0, st>>>(
           (const uint8_t*)a, (const uint8_t*)b, a_s, b_s, c, bias, acc_out, (int)M, (int)N,
-          (int)K, (int)bn, (int)bk);
+          (int)K, (int)bn, (int)bk, LinEpi{});
   });
   return check_launch(fp8 ? "w8a8_block_fp8_matmul (generic)" : "w8a8_block_int8_matmul (generic)");
+}
+
+// The products with an epilogue on the SIMT tiles: float32 operands (a, b fp32; any size, K = 0
+// included), and block sizes the tensor-core kernel does not take.
+int linear_dense_simt_launch(const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
+                             int64_t K, const LinEpi& ep, cudaStream_t st) {
+  if (M > INT32_MAX / 2 || N > INT32_MAX / 2 || K > INT32_MAX / 2)
+    return fail(TO_EUNSUPPORTED, "gemm_bias_act: dimensions too large");
+  dim3 grid((unsigned)ceil_div(N, kTN), (unsigned)ceil_div(M, kTM));
+  if (grid.y > 65535) return fail(TO_EUNSUPPORTED, "gemm_bias_act: M too large for the SIMT tiles");
+  TOB_DISPATCH_FLOAT(ep.dtype, T, {
+    k_gemm_dense_simt<T, true><<<grid, kThreads, 0, st>>>((const T*)a, (const T*)b, nullptr, (int)M,
+                                                           (int)N, (int)K, lda, ep);
+  });
+  return check_launch("gemm_bias_act (SIMT tiles)");
+}
+
+int linear_w8a8_simt_launch(bool fp8, const void* a, const void* b, int64_t M, int64_t N, int64_t K,
+                            int64_t bn, int64_t bk, const LinEpi& ep, cudaStream_t st) {
+  if (M > INT32_MAX / 2 || N > INT32_MAX / 2 || K > INT32_MAX / 2)
+    return fail(TO_EUNSUPPORTED, "w8a8 with epilogue: dimensions too large");
+  dim3 grid((unsigned)ceil_div(N, kTN), (unsigned)ceil_div(M, kTM));
+  if (grid.y > 65535)
+    return fail(TO_EUNSUPPORTED, "w8a8 with epilogue: M too large for the SIMT tiles");
+  TOB_DISPATCH_FLOAT(ep.dtype, TC, {
+    if (fp8)
+      k_w8a8_generic<true, TC, true><<<grid, kThreads, 0, st>>>(
+          (const uint8_t*)a, (const uint8_t*)b, ep.a_s, ep.b_s, nullptr, nullptr, nullptr, (int)M,
+          (int)N, (int)K, (int)bn, (int)bk, ep);
+    else
+      k_w8a8_generic<false, TC, true><<<grid, kThreads, 0, st>>>(
+          (const uint8_t*)a, (const uint8_t*)b, ep.a_s, ep.b_s, nullptr, nullptr, nullptr, (int)M,
+          (int)N, (int)K, (int)bn, (int)bk, ep);
+  });
+  return check_launch("w8a8 with epilogue (SIMT tiles)");
 }
 
 }  // namespace tob

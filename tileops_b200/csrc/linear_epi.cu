@@ -1,0 +1,109 @@
+// Entry points of the products with bias, activation and residual in their epilogue: checks, then
+// the tensor-core tiles (linear_nt_sm100.cu), or the SIMT tiles for what those do not take.
+#include "linear_epi.cuh"
+
+namespace tob {
+namespace sm100 {
+int linear_nt_launch(int kind, bool block_scaled, const void* x, int64_t ldx, const void* w,
+                     int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st);
+}
+int linear_dense_simt_launch(const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
+                             int64_t K, const LinEpi& ep, cudaStream_t st);
+int linear_w8a8_simt_launch(bool fp8, const void* a, const void* b, int64_t M, int64_t N, int64_t K,
+                            int64_t bn, int64_t bk, const LinEpi& ep, cudaStream_t st);
+
+namespace {
+
+// Fills the epilogue common to both products; TO_OK or a recorded failure.
+int make_epi(LinEpi* ep, const char* op, const void* bias, int act, const void* res, int64_t ldr,
+             void* c, int64_t ldc, int dtype, int64_t M, int64_t N) {
+  if (dtype != TO_F32 && dtype != TO_F16 && dtype != TO_BF16)
+    return fail(TO_EUNSUPPORTED, "%s: output dtype %s (float32, float16 and bfloat16)", op,
+                dtype_name(dtype));
+  if (act < kActNone || act > kActGelu)
+    return fail(TO_EINVAL, "%s: unknown activation %d", op, act);
+  if (M > 1 && (ldc < N || (res != nullptr && ldr < N)))
+    return fail(TO_EINVAL, "%s: row strides (%lld, %lld) shorter than N=%lld", op, (long long)ldr,
+                (long long)ldc, (long long)N);
+  if (!c) return fail(TO_EINVAL, "%s: null output", op);
+  ep->bias = bias;
+  ep->res = res;
+  ep->ldr = ldr;
+  ep->c = c;
+  ep->ldc = ldc;
+  ep->dtype = dtype;
+  ep->act = act;
+  return TO_OK;
+}
+
+int w8a8_epi_entry(bool fp8, const void* a, const void* b, const float* a_s, const float* b_s,
+                   const void* bias, int act, const void* res, int64_t ldr, void* c, int64_t ldc,
+                   int c_dtype, int64_t M, int64_t N, int64_t K, int64_t bn, int64_t bk,
+                   void* stream) {
+  const char* op = fp8 ? "w8a8_block_fp8_matmul_bias_act" : "w8a8_block_int8_matmul_bias_act";
+  if (M < 0 || N < 0 || K <= 0 || bn <= 0 || bk <= 0 || M > INT32_MAX || N > INT32_MAX ||
+      K > INT32_MAX)
+    return fail(TO_EINVAL, "%s: invalid M=%lld N=%lld K=%lld block=[%lld,%lld]", op, (long long)M,
+                (long long)N, (long long)K, (long long)bn, (long long)bk);
+  LinEpi ep;
+  if (M == 0 || N == 0) return TO_OK;
+  if (!a || !b || !a_s || !b_s) return fail(TO_EINVAL, "%s: null pointer", op);
+  const int rc = make_epi(&ep, op, bias, act, res, ldr, c, ldc, c_dtype, M, N);
+  if (rc) return rc;
+  const int64_t kt = ceil_div(K, bk);
+  ep.a_s = a_s;
+  ep.b_s = b_s;
+  ep.a_s_ld = ep.b_s_ld = kt;
+  ep.bn = bn >= N ? N : bn;
+  cudaStream_t st = (cudaStream_t)stream;
+  // The tensor-core tiles change scales on whole 128-byte K slices; one K block needs none.
+  if (kt > 1 && bk % 128 != 0)
+    return linear_w8a8_simt_launch(fp8, a, b, M, N, K, ep.bn, bk, ep, st);
+  ep.kb_per_scale = kt > 1 ? (int)(bk / 128) : 1;
+  return sm100::linear_nt_launch(fp8 ? TO_E4M3 : TO_I8, kt > 1, a, K, b, M, N, K, ep, st);
+}
+
+}  // namespace
+}  // namespace tob
+
+extern "C" {
+
+int to_gemm_bias_act(const void* a, int64_t lda, const void* b, const void* bias, int act,
+                     const void* residual, int64_t ldr, void* c, int64_t ldc, int dtype, int64_t M,
+                     int64_t N, int64_t K, void* stream) {
+  using namespace tob;
+  const char* op = "gemm_bias_act";
+  if (M < 0 || N < 0 || K < 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX)
+    return fail(TO_EINVAL, "%s: invalid shape M=%lld N=%lld K=%lld", op, (long long)M,
+                (long long)N, (long long)K);
+  if (M > 1 && lda < K)
+    return fail(TO_EINVAL, "%s: row stride %lld shorter than K=%lld", op, (long long)lda,
+                (long long)K);
+  if (M == 0 || N == 0) return TO_OK;
+  if (K > 0 && (!a || !b)) return fail(TO_EINVAL, "%s: null pointer", op);
+  LinEpi ep;
+  const int rc = make_epi(&ep, op, bias, act, residual, ldr, c, ldc, dtype, M, N);
+  if (rc) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == TO_F32 || K == 0)
+    return linear_dense_simt_launch(a, lda, b, M, N, K, ep, st);
+  return sm100::linear_nt_launch(dtype, false, a, lda, b, M, N, K, ep, st);
+}
+
+int to_w8a8_i8_gemm_bias_act(const int8_t* a, const int8_t* b, const float* a_s, const float* b_s,
+                             const void* bias, int act, const void* residual, int64_t ldr, void* c,
+                             int64_t ldc, int c_dtype, int64_t M, int64_t N, int64_t K,
+                             int64_t block_n, int64_t block_k, void* stream) {
+  return tob::w8a8_epi_entry(false, a, b, a_s, b_s, bias, act, residual, ldr, c, ldc, c_dtype, M, N,
+                             K, block_n, block_k, stream);
+}
+
+int to_w8a8_fp8_gemm_bias_act(const void* a, const void* b, const float* a_s, const float* b_s,
+                              const void* bias, int act, const void* residual, int64_t ldr, void* c,
+                              int64_t ldc, int c_dtype, int64_t M, int64_t N, int64_t K,
+                              int64_t block_n, int64_t block_k, void* stream) {
+  return tob::w8a8_epi_entry(true, a, b, a_s, b_s, bias, act, residual, ldr, c, ldc, c_dtype, M, N,
+                             K, block_n, block_k, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,58 @@
+// Epilogue of the products with bias, activation and residual:
+//   C[m, n] = T( act( acc[m, n] + bias[n] ) + residual[m, n] )
+// acc is the scaled fp32 sum; everything up to the one rounding to T is fp32.
+#pragma once
+
+#include "common.cuh"
+
+namespace tob {
+
+// 0 none, 1 relu, 2 silu, 3 gelu (tanh form): the `act` argument of the C entries.
+enum EpiAct : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3 };
+
+// Both gated forms are x * sigmoid(z): silu with z = x, gelu_tanh with z = 2 sqrt(2/pi)
+// (x + 0.044715 x^3), since (1 + tanh(u)) / 2 = sigmoid(2u). In this form nothing cancels for
+// negative x. FAST takes the hardware exponential and division (relative error about 1e-6 over
+// the range where the result is not negligible, far below half a step of a 16-bit result).
+template <bool FAST>
+__device__ __forceinline__ float x_sigmoid(float x, float z) {
+  if constexpr (FAST) return __fdividef(x, 1.0f + __expf(-z));
+  else return x / (1.0f + expf(-z));
+}
+template <bool FAST>
+__device__ __forceinline__ float epi_act(float x, int act) {
+  if (act == kActNone) return x;
+  if (act == kActRelu) return x < 0.0f ? 0.0f : x;  // NaN stays NaN
+  const float z = act == kActSilu ? x : 1.5957691216057308f * fmaf(0.044715f * x * x, x, x);
+  return x_sigmoid<FAST>(x, z);
+}
+
+// What a product's epilogue reads and writes besides the accumulators. Row strides in elements.
+struct LinEpi {
+  const float* a_s = nullptr;  // scale of token m in K block kb: a_s[m * a_s_ld + kb]; null: 1
+  const float* b_s = nullptr;  // scale of column n: b_s[(n / bn) * b_s_ld + kb]; null: 1
+  int64_t a_s_ld = 0, b_s_ld = 0;
+  int64_t bn = 1;
+  int kb_per_scale = 1;        // 128-byte K slices per scale block (block-scaled products)
+  const void* bias = nullptr;  // [N] of `dtype`, or null
+  const void* res = nullptr;   // [M, N] of `dtype`, rows ldr apart, or null
+  void* c = nullptr;           // [M, N] of `dtype`, rows ldc apart
+  int64_t ldr = 0, ldc = 0;
+  int dtype = TO_F32;
+  int act = kActNone;
+};
+
+// Element i of an array of `dtype` (TO_F32 / TO_F16 / TO_BF16) as fp32, and its store. The
+// residual may be the output itself (in-place add), so its loads stay ordinary loads.
+__device__ __forceinline__ float ld_dtype(const void* p, int64_t i, int dtype) {
+  if (dtype == TO_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  if (dtype == TO_F16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
+  return reinterpret_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void st_dtype(void* p, int64_t i, int dtype, float v) {
+  if (dtype == TO_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else if (dtype == TO_F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+  else reinterpret_cast<float*>(p)[i] = v;
+}
+
+}  // namespace tob

@@ -1,0 +1,608 @@
+// Products with bias, activation and residual in their epilogue, in the orientation "weights as
+// rows": C^T = W X^T, a tile being 128 weight columns of the output x NT tokens. The weights are
+// the 128-row operand of tcgen05.mma and the tokens its N operand, so a single token costs a
+// 16-column tile and not a 128-row one, and the epilogue's lanes run along consecutive output
+// columns: bias and column scale are one register per lane, rows of C and of the residual are
+// read and written coalesced at any alignment.
+//
+//   weights  int8 / e4m3 [N, K] (K-major), or fp16 / bf16 [K, N] (MN-major, 64-column strips)
+//   tokens   [M, K], rows lda apart
+//
+// One token: bound by the weights' HBM stream. The K blocks of a column tile are split over the S
+// CTAs of a cluster so that every SM streams; the partial sums (int32 or fp32) are added through
+// distributed shared memory in rank order (deterministic, no workspace).
+//
+// Operands come by TMA when their rows are 16-byte aligned (PLAIN = false). Any other stride,
+// offset or size takes PLAIN: eight warps load the rows with the widest loads their alignment
+// allows, realign them in registers and store them in the same swizzled layout.
+//
+// Roles: warp 0 weight copies, warp 1 MMA issue and TMEM, warp 2 token copies, warp 3 idle, then
+// kEpiWarps epilogue warps (lane quarter = warp % 4) and, with PLAIN, kLoadWarps loaders.
+// Every wait is bounded (kWaitLimitNs); on expiry all roles unwind through the same barriers.
+#include <cudaTypedefs.h>
+
+#include <string.h>
+
+#include <algorithm>
+
+#include "linear_epi.cuh"
+#include "sm100.cuh"
+
+namespace tob {
+namespace sm100 {
+
+PFN_cuTensorMapEncodeTiled_v12000 get_encode();
+
+namespace {
+
+template <Kind KD, int NT, bool BS, bool PLAIN>
+struct NtCfg {
+  static_assert(NT == 16 || NT == 32 || NT == 64 || NT == 128, "token tile");
+  static constexpr int kElem = KindTraits<KD>::kElemBytes;
+  static constexpr bool kMn = kElem == 2;   // weights [K, N]
+  static constexpr int kBK = 128 / kElem;   // K elements per stage
+  static constexpr int kWBytes = 128 * 128;
+  static constexpr int kXBytes = NT * 128;
+  static constexpr int kStageBytes = kWBytes + kXBytes;
+  static constexpr int kEpiWarps = NT >= 64 ? 8 : 4;
+  static constexpr int kTpt = NT / (kEpiWarps / 4);  // tokens per epilogue thread
+  static constexpr int kLoadWarps = PLAIN ? 8 : 0;
+  static constexpr int kThreads = 128 + 32 * (kEpiWarps + kLoadWarps);
+  // Two CTAs per SM where registers allow: one CTA's prologue and reduction run under the other's
+  // stream. The loaders and the 64 running sums of a 128-token block-scaled tile do not fit twice.
+  static constexpr int kMinBlocks = (PLAIN || (BS && NT == 128)) ? 1 : 2;
+  static constexpr int kStages = (kMinBlocks == 2 ? 110 : 220) * 1024 / kStageBytes;
+  static constexpr int kTmemCols = (BS ? 2 : 1) * NT < 32 ? 32 : (BS ? 2 : 1) * NT;
+  static constexpr size_t kSmem = (size_t)kStages * kStageBytes + 512;
+  static_assert((2 * kStages + 6) * 8 + 16 <= 512, "barrier area");
+  static_assert(128 * NT * 4 <= kStages * kStageBytes, "partial sums reuse the ring");
+  static_assert(kSmem <= 232448, "shared memory");
+};
+
+struct NtArgs {
+  int M, N, K, splits;
+  int strips3d;       // MN-major weights through the 3-D strip map (N % 64 == 0)
+  // PLAIN operands
+  const uint8_t* w;
+  const uint8_t* x;
+  int64_t w_pitch, x_pitch;  // bytes between rows
+  int w_align, x_align;      // largest power of two <= 16 dividing base and pitch
+  LinEpi ep;
+};
+
+// 16 bytes at p, of which the first `valid` (0..16) exist; the rest read as zero. `align` divides
+// p. [lo, hi) is the operand's memory: nothing outside it is touched.
+__device__ __forceinline__ uint4 load_chunk(const uint8_t* p, int valid, int align,
+                                            const uint8_t* lo, const uint8_t* hi) {
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  if (valid >= 16 && align >= 4) {
+    if (align >= 16) return __ldg(reinterpret_cast<const uint4*>(p));
+    if (align == 8) {
+      const uint2 a = __ldg(reinterpret_cast<const uint2*>(p));
+      const uint2 b = __ldg(reinterpret_cast<const uint2*>(p) + 1);
+      return make_uint4(a.x, a.y, b.x, b.y);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+  } else if (valid > 0) {
+    // Aligned words around p, shifted together. A word that would reach outside the operand, or
+    // past the row's valid bytes, is assembled from single bytes.
+    const int sh = (int)(reinterpret_cast<uintptr_t>(p) & 3u);
+    const uint8_t* base = p - sh;
+    if (valid >= 16 && base >= lo && base + 20 <= hi) {
+      uint32_t r[5];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = __ldg(reinterpret_cast<const uint32_t*>(base) + i);
+      r[4] = sh ? __ldg(reinterpret_cast<const uint32_t*>(base) + 4) : 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(r[i], r[i + 1], 8 * sh);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (i < valid) w[i / 4] |= (uint32_t)__ldg(p + i) << (8 * (i % 4));
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <Kind KD, int NT, bool BS, bool PLAIN>
+__global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
+                                  NtCfg<KD, NT, BS, PLAIN>::kMinBlocks)
+    k_linear_nt(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                const __grid_constant__ NtArgs g, int* err) {
+  using C = NtCfg<KD, NT, BS, PLAIN>;
+  using Tr = KindTraits<KD>;
+  constexpr int ST = C::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* sW = smem_raw;
+  uint8_t* sX = smem_raw + (size_t)ST * C::kWBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw + (size_t)ST * C::kStageBytes);
+  uint64_t* empty = full + ST;
+  uint64_t* tfull = empty + ST;   // [2]; unscaled products use tfull[0]
+  uint64_t* tempty = tfull + 2;   // [2]
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int S = g.splits;
+  const int rank = (int)blockIdx.x % S;
+  const int n0 = ((int)blockIdx.x / S) * 128;
+  const int t0 = (int)blockIdx.y * NT;
+  const int tokens = min(NT, g.M - t0);
+  const int kblocks = (g.K + C::kBK - 1) / C::kBK;
+  const int kb_lo = (int)((int64_t)kblocks * rank / S);
+  const int kb_n = (int)((int64_t)kblocks * (rank + 1) / S) - kb_lo;
+  const bool misaligned = (smem_u32(smem_raw) & 1023u) != 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(full + s, PLAIN ? C::kLoadWarps : 2);
+      mbar_init(empty + s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull + b, 1);
+      mbar_init(tempty + b, C::kEpiWarps);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    if (!PLAIN) {
+      prefetch_tmap(&tmW);
+      prefetch_tmap(&tmX);
+    }
+    if (misaligned && err) atomicExch(err, (int)kErrSmemAlign);
+  }
+  if (warp == 1) tmem_alloc<C::kTmemCols>(tmem_holder);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  bool ok = !misaligned;
+
+  if (!ok) {
+    // nothing to do; fall through to the barriers and the teardown
+  } else if (!PLAIN && (warp == 0 || warp == 2)) {
+    // ------------------------------------------------------------ TMA: weights / tokens
+    if (lane == 0) {
+      const bool wts = warp == 0;
+      // The weights stream once past L2's other contents; every column tile re-reads the tokens.
+      const uint64_t pol = wts ? policy_evict_first() : policy_evict_last();
+      if (!wts) grid_dependency_wait();  // the tokens may be the previous kernel's output
+      uint32_t issued_mask = 0, issued_phase = 0;
+      for (int it = 0; it < kb_n; ++it) {
+        const int s = it % ST;
+        const uint32_t ph = (uint32_t)(it / ST) & 1u;
+        const int k = (kb_lo + it) * C::kBK;
+        if (it >= ST && !mbar_wait(empty + s, ph ^ 1, abort_flag, err)) { ok = false; break; }
+        mbar_arrive_expect_tx(full + s, wts ? C::kWBytes : C::kXBytes);
+        if (!wts) {
+          tma_load_2d(sX + (size_t)s * C::kXBytes, &tmX, k, t0, full + s, pol);
+        } else if (!C::kMn) {
+          tma_load_2d(sW + (size_t)s * C::kWBytes, &tmW, k, n0, full + s, pol);
+        } else if (g.strips3d) {
+          tma_load_3d(sW + (size_t)s * C::kWBytes, &tmW, 0, k, n0 / 64, full + s, pol);
+        } else {
+          tma_load_2d(sW + (size_t)s * C::kWBytes, &tmW, n0, k, full + s, pol);
+          tma_load_2d(sW + (size_t)s * C::kWBytes + 8192, &tmW, n0 + 64, k, full + s, pol);
+        }
+        issued_mask |= 1u << s;
+        issued_phase = (issued_phase & ~(1u << s)) | (ph << s);
+      }
+      if (ok) {
+        if (wts) grid_dependents_launch();
+      } else {
+        // Unwinding: let the copies in flight land before the CTA exits (one deadline).
+        const uint64_t tw = globaltimer_ns();
+        for (int i = 0; i < ST; ++i)
+          if (issued_mask & (1u << i))
+            while (!mbar_try_wait(full + i, (issued_phase >> i) & 1u) &&
+                   globaltimer_ns() - tw < kWaitLimitNs) {
+            }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc =
+          make_idesc_major(Tr::kDFmt, Tr::kAFmt, Tr::kBFmt, 128, NT, C::kMn ? 1 : 0, 0);
+      bool any = false;
+      for (int it = 0; it < kb_n; ++it) {
+        const int s = it % ST;
+        if (!mbar_wait(full + s, (uint32_t)(it / ST) & 1u, abort_flag, err)) { ok = false; break; }
+        const int b = BS ? it & 1 : 0;
+        if (BS && it >= 2 &&
+            !mbar_wait(tempty + b, ((uint32_t)(it >> 1) & 1u) ^ 1, abort_flag, err)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t w0 = smem_u32(sW + (size_t)s * C::kWBytes);
+        const uint32_t x0 = smem_u32(sX + (size_t)s * C::kXBytes);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // MN-major: 64-column strips of 64 K rows (8 KB apart); 16 K rows are 2 KB
+          const uint64_t wd = C::kMn ? smem_desc_mnmajor_sw128(w0 + 2048 * k, 8192, 1024)
+                                     : smem_desc_kmajor_sw128(w0 + 32 * k);
+          umma<KD>(tmem + (uint32_t)(b * NT), wd, smem_desc_kmajor_sw128(x0 + 32 * k), idesc,
+                   BS ? k != 0 : (it | k) != 0);
+        }
+        any = true;
+        umma_commit(empty + s);
+        if (BS) umma_commit(tfull + b);
+      }
+      if (ok && !BS) umma_commit(tfull);
+      if (!ok && any) {
+        // Unwinding: wait (bounded) until the MMAs already issued have finished with TMEM.
+        umma_commit(drain);
+        const uint64_t tw = globaltimer_ns();
+        while (!mbar_try_wait(drain, 0) && globaltimer_ns() - tw < kWaitLimitNs) {
+        }
+      }
+    }
+  } else if (PLAIN && warp >= 4 + C::kEpiWarps) {
+    // ------------------------------------------------------------ loaders (any alignment)
+    if constexpr (PLAIN) {
+      // A warp takes groups of four 128-byte rows, a lane one 16-byte chunk of a row.
+      constexpr int kGroups = (128 + NT) / 4;
+      constexpr int kMine = (kGroups + C::kLoadWarps - 1) / C::kLoadWarps;
+      const int lw = warp - 4 - C::kEpiWarps;
+      const int chunk = lane & 7;
+      const int64_t row_bytes = (int64_t)g.K * C::kElem;
+      const int64_t w_rows = C::kMn ? g.K : g.N;
+      const int64_t w_bytes = C::kMn ? (int64_t)g.N * 2 : row_bytes;
+      const uint8_t* w_hi = g.w + (w_rows - 1) * g.w_pitch + w_bytes;
+      const uint8_t* x_hi = g.x + (int64_t)(g.M - 1) * g.x_pitch + row_bytes;
+      grid_dependency_wait();
+      for (int it = 0; it < kb_n; ++it) {
+        const int s = it % ST;
+        const int64_t kbyte = (int64_t)(kb_lo + it) * 128;
+        uint4 v[kMine];
+  #pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int row = (lw + i * C::kLoadWarps) * 4 + (lane >> 3);
+          v[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (row < 128) {
+            int64_t r, off;  // source row and byte offset in it
+            if (C::kMn) {
+              r = (int64_t)(kb_lo + it) * 64 + (row & 63);
+              off = (int64_t)(n0 + (row & 64)) * 2 + chunk * 16;
+            } else {
+              r = n0 + row;
+              off = kbyte + chunk * 16;
+            }
+            if (r < w_rows && off < w_bytes)
+              v[i] = load_chunk(g.w + r * g.w_pitch + off, (int)min((int64_t)16, w_bytes - off),
+                                g.w_align, g.w, w_hi);
+          } else if (row < 128 + NT) {
+            const int t = row - 128;
+            const int64_t off = kbyte + chunk * 16;
+            if (t < tokens && off < row_bytes)
+              v[i] = load_chunk(g.x + (int64_t)(t0 + t) * g.x_pitch + off,
+                                (int)min((int64_t)16, row_bytes - off), g.x_align, g.x, x_hi);
+          }
+        }
+        if (it >= ST && !mbar_wait(empty + s, ((uint32_t)(it / ST) & 1u) ^ 1, abort_flag, err)) {
+          ok = false;
+          break;
+        }
+  #pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int row = (lw + i * C::kLoadWarps) * 4 + (lane >> 3);
+          if (row >= 128 + NT) continue;
+          uint8_t* tile = row < 128 ? sW + (size_t)s * C::kWBytes : sX + (size_t)s * C::kXBytes;
+          const int r = row < 128 ? row : row - 128;
+          *reinterpret_cast<uint4*>(tile + r * 128 + ((chunk ^ (r & 7)) << 4)) = v[i];
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + s);
+      }
+    }
+  }
+
+  // -------------------------------------------------------------- epilogue
+  const bool epi = warp >= 4 && warp < 4 + C::kEpiWarps;
+  const int q = warp & 3;                     // TMEM lane quarter
+  const int half = (warp - 4) >> 2;           // which kTpt tokens of the tile
+  const int n = n0 + q * 32 + lane;
+  const bool n_ok = n < g.N;
+  const LinEpi& ep = g.ep;
+  float* part = reinterpret_cast<float*>(smem_raw);  // [token][128] partial sums (ring reuse)
+  float bias = 0.f, sb = 1.f, sa_l[(C::kTpt + 31) / 32];
+  // One output value; every lane of the warp calls it (shuffled token scale).
+  auto finish = [&](float acc, float sa, int tok, float res) {
+    float v = BS ? acc : acc * (sa * sb);
+    v = epi_act<true>(v + bias, ep.act) + res;
+    if (n_ok) st_dtype(ep.c, (int64_t)(t0 + tok) * ep.ldc + n, ep.dtype, v);
+  };
+  if (epi && ok) {
+    grid_dependency_wait();
+    if (n_ok && ep.bias != nullptr) bias = ld_dtype(ep.bias, n, ep.dtype);
+    const int64_t brow = (n_ok ? (int64_t)n / ep.bn : 0) * ep.b_s_ld;
+    if (!BS && ep.b_s != nullptr && n_ok) sb = __ldg(ep.b_s + brow);
+    const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * C::kTpt);
+    if constexpr (BS) {
+      float run[C::kTpt];
+#pragma unroll
+      for (int j = 0; j < C::kTpt; ++j) run[j] = 0.f;
+      for (int it = 0; it < kb_n; ++it) {
+        const int kb = (kb_lo + it) / ep.kb_per_scale;
+        const float s_col = n_ok ? __ldg(ep.b_s + brow + kb) : 0.f;
+#pragma unroll
+        for (int i = 0; i < (C::kTpt + 31) / 32; ++i) {
+          const int t = half * C::kTpt + i * 32 + lane;
+          sa_l[i] = t < tokens ? __ldg(ep.a_s + (int64_t)(t0 + t) * ep.a_s_ld + kb) : 0.f;
+        }
+        const int b = it & 1;
+        if (!mbar_wait(tfull + b, (uint32_t)(it >> 1) & 1u, abort_flag, err)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < C::kTpt; c += 16) {
+          uint32_t r[16];
+          tmem_ld16(lane_addr + (uint32_t)(b * NT + c), r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float p = KD == Kind::I8 ? (float)(int32_t)r[j] : __uint_as_float(r[j]);
+            const float sa = __shfl_sync(0xffffffffu, sa_l[(c + j) / 32], (c + j) & 31);
+            run[c + j] = fmaf(p * sa, s_col, run[c + j]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tempty + b);
+      }
+      if (ok) {
+        if (S > 1) {
+          // The ring is idle only once every MMA of this CTA has read its operands: the last
+          // tfull covers them all.
+#pragma unroll
+          for (int j = 0; j < C::kTpt; ++j)
+            part[(half * C::kTpt + j) * 128 + q * 32 + lane] = run[j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < C::kTpt; ++j) {
+            const int tok = half * C::kTpt + j;
+            if (tok >= tokens) break;
+            float res = 0.f;
+            if (ep.res != nullptr && n_ok)
+              res = ld_dtype(ep.res, (int64_t)(t0 + tok) * ep.ldr + n, ep.dtype);
+            finish(run[j], 1.f, tok, res);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < (C::kTpt + 31) / 32; ++i) {
+        const int t = half * C::kTpt + i * 32 + lane;
+        sa_l[i] = ep.a_s != nullptr && t < tokens ? __ldg(ep.a_s + (int64_t)(t0 + t) * ep.a_s_ld)
+                                                  : 1.f;
+      }
+#pragma unroll
+      for (int c = 0; c < C::kTpt; c += 16) {
+        const int tok0 = half * C::kTpt + c;
+        float res[16];
+        const bool direct = S == 1;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          res[j] = 0.f;
+          if (direct && ep.res != nullptr && n_ok && tok0 + j < tokens)
+            res[j] = ld_dtype(ep.res, (int64_t)(t0 + tok0 + j) * ep.ldr + n, ep.dtype);
+        }
+        if (c == 0) {
+          ok = mbar_wait(tfull, 0, abort_flag, err);
+          tc_fence_after();
+        }
+        if (!ok) break;
+        if (tok0 >= tokens) break;
+        uint32_t r[16];
+        tmem_ld16(lane_addr + (uint32_t)c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int tok = tok0 + j;
+          if (S > 1) {
+            reinterpret_cast<uint32_t*>(part)[tok * 128 + q * 32 + lane] = r[j];
+          } else {
+            const float sa = __shfl_sync(0xffffffffu, sa_l[(c + j) / 32], (c + j) & 31);
+            const float a = KD == Kind::I8 ? (float)(int32_t)r[j] : __uint_as_float(r[j]);
+            if (tok < tokens) finish(a, sa, tok, res[j]);
+          }
+        }
+      }
+    }
+  }
+  if (S > 1) {
+    cluster_sync_all();  // every rank's partial sums are in its shared memory
+    if (epi && ok) {
+      // Rank r finishes tokens r, r + S, ...; the sums run over the ranks in order.
+      const uint32_t mine = smem_u32(part + q * 32 + lane);
+      for (int i = half; rank + i * S < tokens; i += C::kEpiWarps / 4) {
+        const int tok = rank + i * S;
+        float res = 0.f;
+        if (ep.res != nullptr && n_ok)
+          res = ld_dtype(ep.res, (int64_t)(t0 + tok) * ep.ldr + n, ep.dtype);
+        float sa = 1.f;
+        if (!BS && ep.a_s != nullptr) sa = __ldg(ep.a_s + (int64_t)(t0 + tok) * ep.a_s_ld);
+        uint32_t v[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          v[s] = 0u;
+          if (s < S) {
+            const uint32_t addr = mapa_shared(mine + (uint32_t)tok * 512u, (uint32_t)s);
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v[s]) : "r"(addr) : "memory");
+          }
+        }
+        float acc;
+        if (KD == Kind::I8 && !BS) {
+          int32_t t = 0;
+#pragma unroll
+          for (int s = 0; s < 8; ++s) t += (int32_t)v[s];
+          acc = (float)t;
+        } else {
+          acc = __uint_as_float(v[0]);
+#pragma unroll
+          for (int s = 1; s < 8; ++s)
+            if (s < S) acc += __uint_as_float(v[s]);
+        }
+        finish(acc, sa, tok, res);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<C::kTmemCols>(tmem);
+  }
+  if (S > 1) cluster_sync_all();  // no rank leaves while a peer still reads its partial sums
+}
+
+// 2-D map of `rows` x `cols` elements, rows `pitch` bytes apart, boxes of 128 bytes x box_rows in
+// the 128-byte swizzle. Built per call: it costs well under a microsecond.
+int rows_map(CUtensorMap* out, const void* p, int64_t rows, int64_t cols, int64_t pitch, int elem,
+             int box_rows) {
+  auto encode = get_encode();
+  if (!encode) return fail(TO_ECUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)pitch};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / elem), (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = encode(
+      out, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
+      const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(TO_ECUDA, "cuTensorMapEncodeTiled failed (%d) for [%lld, %lld]", (int)r,
+                (long long)rows, (long long)cols);
+  return TO_OK;
+}
+
+// Weights [K, N], N % 64 == 0, as {64 columns, K rows, N / 64 strips}: one box of two strips.
+int strips_map(CUtensorMap* out, const void* p, int64_t K, int64_t N) {
+  auto encode = get_encode();
+  if (!encode) return fail(TO_ECUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  cuuint64_t dims[3] = {64, (cuuint64_t)K, (cuuint64_t)(N / 64)};
+  cuuint64_t strides[2] = {(cuuint64_t)(N * 2), 128};
+  cuuint32_t box[3] = {64, 64, 2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(p), dims,
+                            strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(TO_ECUDA, "cuTensorMapEncodeTiled (strips) failed (%d) for [%lld, %lld]", (int)r,
+                (long long)K, (long long)N);
+  return TO_OK;
+}
+
+int pow2_align(const void* p, int64_t pitch) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p) | (uint64_t)pitch | 16u;
+  return (int)(v & (~v + 1));
+}
+
+template <Kind KD, int NT, bool BS, bool PLAIN>
+int launch_nt(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, int64_t K,
+              const LinEpi& ep, cudaStream_t st) {
+  using C = NtCfg<KD, NT, BS, PLAIN>;
+  auto kern = k_linear_nt<KD, NT, BS, PLAIN>;
+  const cudaError_t ae = ensure_smem_attr((const void*)kern, (int)C::kSmem);
+  if (ae != cudaSuccess) return cuda_fail(ae, "linear epilogue: shared memory attribute");
+  const int64_t n_tiles = ceil_div(N, 128), m_tiles = ceil_div(M, NT);
+  const int64_t kblocks = ceil_div(K, C::kBK);
+  // K split: as many CTAs as the SMs hold at once, at least two K blocks each, at most a
+  // portable cluster of eight.
+  const int64_t slots = (int64_t)sm_count() * C::kMinBlocks;
+  int64_t S = slots / (n_tiles * m_tiles);
+  S = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(S, 8), kblocks / 2));
+  if (n_tiles * S > INT32_MAX || m_tiles > 65535)
+    return fail(TO_EUNSUPPORTED, "linear epilogue: too many tiles (M=%lld N=%lld)", (long long)M,
+                (long long)N);
+  NtArgs g;
+  memset((void*)&g, 0, sizeof(g));
+  g.M = (int)M;
+  g.N = (int)N;
+  g.K = (int)K;
+  g.splits = (int)S;
+  g.strips3d = C::kMn && N % 64 == 0;
+  g.w = (const uint8_t*)w;
+  g.x = (const uint8_t*)x;
+  g.w_pitch = (C::kMn ? N : K) * C::kElem;
+  g.x_pitch = ldx * C::kElem;
+  g.w_align = pow2_align(w, g.w_pitch);
+  g.x_align = pow2_align(x, g.x_pitch);
+  g.ep = ep;
+  CUtensorMap tw, tx;
+  memset(&tw, 0, sizeof(tw));
+  memset(&tx, 0, sizeof(tx));
+  if (!PLAIN) {
+    int rc = !C::kMn      ? rows_map(&tw, w, N, K, g.w_pitch, C::kElem, 128)
+             : g.strips3d ? strips_map(&tw, w, K, N)
+                          : rows_map(&tw, w, K, N, g.w_pitch, C::kElem, 64);
+    if (!rc) rc = rows_map(&tx, x, M, K, g.x_pitch, C::kElem, NT);
+    if (rc) return rc;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(n_tiles * S), (unsigned)m_tiles, 1);
+  cfg.blockDim = dim3(C::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)S;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (launch_overlap()) {
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, tx, g, device_error_ptr());
+  if (e != cudaSuccess) return cuda_fail(e, "linear epilogue launch");
+  return check_launch("linear epilogue");
+}
+
+template <Kind KD, bool BS, bool PLAIN>
+int launch_nt_tokens(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, int64_t K,
+                     const LinEpi& ep, cudaStream_t st) {
+  if (M <= 16) return launch_nt<KD, 16, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
+  if (M <= 32) return launch_nt<KD, 32, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
+  if (M <= 64) return launch_nt<KD, 64, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
+  return launch_nt<KD, 128, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
+}
+
+template <Kind KD, bool BS>
+int launch_nt_any(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, int64_t K,
+                  const LinEpi& ep, cudaStream_t st) {
+  constexpr int e = KindTraits<KD>::kElemBytes;
+  const int64_t w_pitch = (e == 2 ? N : K) * e;
+  const bool tma = pow2_align(w, w_pitch) == 16 && pow2_align(x, ldx * e) == 16;
+  return tma ? launch_nt_tokens<KD, BS, false>(x, ldx, w, M, N, K, ep, st)
+             : launch_nt_tokens<KD, BS, true>(x, ldx, w, M, N, K, ep, st);
+}
+
+}  // namespace
+
+// Entry of this file: `kind` one of TO_I8, TO_E4M3 (weights [N, K]), TO_F16, TO_BF16 (weights
+// [K, N]); block_scaled: ep's scales change every ep.kb_per_scale 128-byte K slices.
+int linear_nt_launch(int kind, bool block_scaled, const void* x, int64_t ldx, const void* w,
+                     int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st) {
+  switch (kind) {
+    case TO_F16: return launch_nt_any<Kind::F16, false>(x, ldx, w, M, N, K, ep, st);
+    case TO_BF16: return launch_nt_any<Kind::BF16, false>(x, ldx, w, M, N, K, ep, st);
+    case TO_I8:
+      return block_scaled ? launch_nt_any<Kind::I8, true>(x, ldx, w, M, N, K, ep, st)
+                          : launch_nt_any<Kind::I8, false>(x, ldx, w, M, N, K, ep, st);
+    case TO_E4M3:
+      return block_scaled ? launch_nt_any<Kind::E4M3, true>(x, ldx, w, M, N, K, ep, st)
+                          : launch_nt_any<Kind::E4M3, false>(x, ldx, w, M, N, K, ep, st);
+  }
+  return fail(TO_EUNSUPPORTED, "linear epilogue: operand dtype %s", dtype_name(kind));
+}
+
+}  // namespace sm100
+}  // namespace tob

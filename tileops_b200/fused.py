@@ -149,4 +149,87 @@ def act_and_mul_group_quant(a: torch.Tensor, b: torch.Tensor, group_size: int, *
     return q, s
 
 
-__all__ = ["act_and_mul_group_quant", "gelu_and_mul", "silu_and_mul"]
+def add_rms_norm_group_quant(x: torch.Tensor, weight: torch.Tensor, group_size: int,
+                             residual: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
+                             dtype: Optional[torch.dtype] = None, quant_eps: float = 1e-10,
+                             column_major_scales: bool = False, use_ue8m0: bool = False,
+                             residual_out: Optional[torch.Tensor] = None):
+    """Library extension (no reference counterpart): the residual's addition, a root-mean-square
+    norm and the per-token-group quantiser in one kernel -- the input of a W8A8 linear straight
+    from the residual stream:
+
+        h = x + residual;  y = h / sqrt(mean(h^2) + eps) * weight        (over the last dimension)
+        scale = max(max|y|, quant_eps) / qmax per group,  q = code(y / scale)
+
+    ``dtype`` torch.float8_e4m3fn (default; qmax 448, optionally power-of-two scales) or
+    torch.int8 (qmax 127); ``group_size`` divides the last dimension and may be all of it. All of
+    it is fp32: unlike an unfused chain, y is not rounded to ``x.dtype`` before it is quantised.
+    ``x``, ``weight`` (one per column) and ``residual`` share a dtype (float32, float16, bfloat16).
+
+    Returns ``(q, scales)``, or ``(q, scales, h)`` with a residual, h rounded to ``x.dtype``:
+    written to ``residual_out`` when given, which may be ``x`` or ``residual`` itself. A row with
+    a NaN has NaN scales, e4m3 NaN codes and int8 zeros; a row of zeros has codes 0 and scales
+    quant_eps / qmax."""
+    op = "add_rms_norm_group_quant"
+    if x.dim() == 0 or tuple(weight.shape) != (x.shape[-1],):
+        raise ValueError(f"{op}: weight.shape={tuple(weight.shape)} does not match the last "
+                         f"dimension of x {tuple(x.shape)}")
+    cols = x.shape[-1]
+    if group_size <= 0 or cols % group_size != 0:
+        raise ValueError(f"{op}: the last dimension of `x` {cols} must be divisible by "
+                         f"`group_size` {group_size}")
+    dtype = torch.float8_e4m3fn if dtype is None else dtype
+    if dtype not in (torch.float8_e4m3fn, torch.int8):
+        raise TypeError(f"{op}: codes must be torch.float8_e4m3fn or torch.int8 (got {dtype})")
+    if dtype == torch.int8 and (use_ue8m0 or column_major_scales):
+        raise ValueError(f"{op}: use_ue8m0 and column_major_scales are FP8 options")
+    if column_major_scales and x.dim() != 2:
+        raise ValueError(f"{op}: column_major_scales needs a 2-D input")
+    if residual_out is not None and residual is None:
+        raise ValueError(f"{op}: residual_out needs a residual")
+    xd = x.dtype
+    for name, t in (("weight", weight), ("residual", residual), ("residual_out", residual_out)):
+        if t is None:
+            continue
+        if name != "weight" and t.shape != x.shape:
+            raise ValueError(f"{op}: {name}.shape={tuple(t.shape)} != x.shape={tuple(x.shape)}")
+        if t.dtype != xd:
+            raise TypeError(f"{op}: {name}.dtype={t.dtype} != x.dtype={xd}")
+        if t.device != x.device:
+            raise TypeError(f"{op}: all tensors must be on {x.device} ({name} is on {t.device})")
+    idx = _lib.ensure_device(x, op)
+    if xd not in _DTYPES:
+        raise TypeError(f"{op}: unsupported dtype {xd} (float32, float16 and bfloat16 are "
+                        "supported)")
+    rows = x.numel() // cols if cols else 0
+    ldx = _row_stride(x)
+    ldr = ldh = 0
+    dst = None
+    if residual is not None:
+        ldr = _row_stride(residual)
+        ldh = None if residual_out is None else _row_stride(residual_out)
+        if ldh is None:
+            dst, ldh = torch.empty(x.shape, dtype=xd, device=x.device), cols
+        else:
+            dst = residual_out
+        if ldr is None:
+            residual, ldr = residual.contiguous(), cols
+    if ldx is None:
+        x, ldx = x.contiguous(), cols
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    q = torch.empty(x.shape, dtype=dtype, device=x.device)
+    s = torch.empty(*x.shape[:-1], cols // group_size, dtype=torch.float32, device=x.device)
+    _lib.call("to_add_rms_norm_group_quant", x.data_ptr(), ldx, _lib.ptr(residual), ldr,
+              weight.data_ptr(), _lib.DTYPE_CODES[xd], rows, cols, group_size, eps, quant_eps,
+              1 if use_ue8m0 else 0, 1 if column_major_scales else 0, _lib.DTYPE_CODES[dtype],
+              q.data_ptr(), s.data_ptr(), _lib.ptr(dst), ldh, _lib.stream_ptr(idx))
+    if residual is None:
+        return q, s
+    if residual_out is not None and dst is not residual_out:
+        residual_out.copy_(dst)
+        dst = residual_out
+    return q, s, dst
+
+
+__all__ = ["act_and_mul_group_quant", "add_rms_norm_group_quant", "gelu_and_mul", "silu_and_mul"]

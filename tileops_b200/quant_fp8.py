@@ -15,7 +15,13 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .quant_int8 import _FLOATS, _run_w8a8, _validate_w8a8, _validate_w8a8_rest
+from .quant_int8 import (
+    _FLOATS,
+    _run_w8a8,
+    _run_w8a8_bias_act,
+    _validate_w8a8,
+    _validate_w8a8_rest,
+)
 
 _FP8_DTYPES = tuple(
     d for d in (getattr(torch, "float8_e4m3fn", None), getattr(torch, "float8_e4m3fnuz", None))
@@ -252,6 +258,36 @@ def w8a8_block_fp8_matmul(
                      output_dtype)
 
 
+def w8a8_block_fp8_matmul_bias_act(
+    a: torch.Tensor,
+    b: torch.Tensor,
+    a_s: torch.Tensor,
+    b_s: torch.Tensor,
+    block_size: list[int],
+    bias: Optional[torch.Tensor] = None,
+    *,
+    act: Optional[str] = None,
+    residual: Optional[torch.Tensor] = None,
+    output_dtype: torch.dtype = torch.float16,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Library extension: ``act(w8a8_block_fp8_matmul(...) + bias) + residual`` in one kernel,
+    everything after the products in fp32 and rounded once to ``output_dtype`` (which bias (N,),
+    residual (..., N) and out share). ``act`` as in :func:`gemm_bias_act`; ``out`` may be
+    ``residual``."""
+    op = "w8a8_block_fp8_matmul_bias_act"
+    block_n, block_k = _validate_w8a8(op, a, b, a_s, b_s, block_size)
+    if not is_fp8(a) or not is_fp8(b):
+        raise TypeError(f"{op}: A and B must be FP8")
+    if a.shape[-1] == 0:
+        raise ValueError(f"{op}: K must be positive")
+    m, n, k = _validate_w8a8_rest(op, a, b, a_s, b_s, block_n, block_k)
+    _require_e4m3fn(a.dtype, op)
+    _require_e4m3fn(b.dtype, op)
+    return _run_w8a8_bias_act("to_w8a8_fp8_gemm_bias_act", op, a, b, a_s, b_s, block_n, block_k, m,
+                              n, k, bias, act, residual, output_dtype, out)
+
+
 def w8a8_triton_block_scaled_mm(
     a: torch.Tensor,
     b: torch.Tensor,
@@ -302,5 +338,6 @@ __all__ = [
     "per_token_group_quant_fp8",
     "per_token_group_quant_fp8_tma_aligned",
     "w8a8_block_fp8_matmul",
+    "w8a8_block_fp8_matmul_bias_act",
     "w8a8_triton_block_scaled_mm",
 ]

@@ -14,7 +14,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from . import _epilogue, _lib
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -231,6 +231,56 @@ def w8a8_block_int8_matmul(
                      output_dtype)
 
 
+def _run_w8a8_bias_act(entry, op, a, b, a_s, b_s, block_n, block_k, m, n, k, bias, act, residual,
+                       output_dtype, out):
+    """C = act(dequant(A) @ dequant(B).T + bias) + residual through one of the C entries."""
+    if output_dtype not in _FLOATS:
+        raise TypeError(f"{op}: output_dtype {output_dtype} (float32, float16, bfloat16)")
+    shape = (*a.shape[:-1], n)
+    device = a.device
+    code = _epilogue.check(op, shape, n, output_dtype, device, bias, act, residual, out)
+    idx = _lib.ensure_device(a, op)
+    _lib.same_device(op, a, b, a_s, b_s)
+    if a_s.dtype != torch.float32 or not a_s.is_contiguous():
+        a_s = a_s.to(torch.float32).contiguous()
+    if b_s.dtype != torch.float32 or not b_s.is_contiguous():
+        b_s = b_s.to(torch.float32).contiguous()
+    bias, residual, ldr, dst, ldc = _epilogue.prepare(shape, n, output_dtype, device, bias,
+                                                      residual, out)
+    _lib.call(entry, a.data_ptr(), b.data_ptr(), a_s.data_ptr(), b_s.data_ptr(), _lib.ptr(bias),
+              code, _lib.ptr(residual), ldr, dst.data_ptr(), ldc,
+              _lib.DTYPE_CODES[output_dtype], m, n, k, block_n, block_k, _lib.stream_ptr(idx))
+    return _epilogue.finish(dst, out)
+
+
+def w8a8_block_int8_matmul_bias_act(
+    a: torch.Tensor,
+    b: torch.Tensor,
+    a_s: torch.Tensor,
+    b_s: torch.Tensor,
+    block_size: list[int],
+    bias: Optional[torch.Tensor] = None,
+    *,
+    act: Optional[str] = None,
+    residual: Optional[torch.Tensor] = None,
+    output_dtype: torch.dtype = torch.float16,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Library extension: ``act(w8a8_block_int8_matmul(...) + bias) + residual`` in one kernel,
+    everything after the int32 block sums in fp32 and rounded once to ``output_dtype`` (which
+    bias (N,), residual (..., N) and out share). ``act`` as in :func:`gemm_bias_act`; ``out`` may
+    be ``residual``."""
+    op = "w8a8_block_int8_matmul_bias_act"
+    block_n, block_k = _validate_w8a8(op, a, b, a_s, b_s, block_size)
+    if a.dtype != torch.int8 or b.dtype != torch.int8:
+        raise TypeError(f"{op}: A and B must be int8")
+    if a.shape[-1] == 0:
+        raise ValueError(f"{op}: K must be positive")
+    m, n, k = _validate_w8a8_rest(op, a, b, a_s, b_s, block_n, block_k)
+    return _run_w8a8_bias_act("to_w8a8_i8_gemm_bias_act", op, a, b, a_s, b_s, block_n, block_k, m,
+                              n, k, bias, act, residual, output_dtype, out)
+
+
 def w8a8_int8_accumulators(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     """Exact int32 ``A @ B.T`` of int8 operands (the accumulators of
     :func:`w8a8_block_int8_matmul`), exposed so they can be checked bit for bit."""
@@ -285,4 +335,5 @@ __all__ = [
     "per_token_group_quant_int8",
     "per_token_quant_int8",
     "w8a8_block_int8_matmul",
+    "w8a8_block_int8_matmul_bias_act",
 ]
