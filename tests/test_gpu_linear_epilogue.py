@@ -353,3 +353,60 @@ def test_offsets_past_32_bits(cuda):
         want = (k * a[rows, :1].float() * b[:1].float()
                 + (torch.arange(n, device=cuda) % 3).float()).bfloat16()
         assert torch.equal(y[rows], want)
+
+
+# Many tokens: several tiles per CTA pair, ragged last tiles, K of one slice, of an odd number of
+# slices, of no whole slice; tile widths chosen by the number of tiles.
+LARGE_SHAPES = [
+    (256, 11008, 512), (257, 9480, 192), (512, 4096, 128), (1000, 6152, 320), (1024, 5120, 136),
+    (2048, 2304, 1024), (2500, 4104, 72), (4100, 2048, 64), (300, 28672, 256), (9000, 640, 200),
+]
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", LARGE_SHAPES)
+def test_dense_exact_many_tokens(cuda, dt, m, n, k):
+    gen = torch.Generator(device=cuda).manual_seed(m + n + k)
+
+    def ri(lo, hi, *shape):
+        return torch.randint(lo, hi + 1, shape, generator=gen, device=cuda).to(dt)
+
+    a, b, bias, res = ri(-3, 3, m, k), ri(-2, 2, k, n), ri(-8, 8, n), ri(-8, 8, m, n)
+    assert torch.equal(tob.gemm_bias_act(a, b), exact_dense(a, b, None, None, None).to(dt))
+    want = exact_dense(a, b, bias, "relu", res).to(dt)
+    y = tob.gemm_bias_act(a, b, bias, act="relu", residual=res)
+    assert torch.equal(y, want)
+    wide = torch.full((m, n + 16), 7, dtype=dt, device=cuda)
+    wide[:, 8:n + 8] = res
+    o = wide[:, 8:n + 8]
+    assert tob.gemm_bias_act(a, b, bias, act="relu", residual=o, out=o) is o
+    assert torch.equal(o, want)
+    assert bool((wide[:, :8] == 7).all()) and bool((wide[:, n + 8:] == 7).all())
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("scales", ["channel", "tensor", "block128", "wide_n", "block256"])
+@pytest.mark.parametrize("m,n,k", LARGE_SHAPES)
+def test_w8a8_exact_many_tokens(cuda, codes, scales, m, n, k):
+    gen = torch.Generator(device=cuda).manual_seed(m + n + k)
+    k = -(-k // 16) * 16
+    bn, bk = {"channel": (1, k), "tensor": (n, k), "block128": (128, 128), "wide_n": (n, 128),
+              "block256": (256, 256)}[scales]
+    hi = 127 if codes == "int8" else 8
+    hi_b = 3 if codes == "int8" else 8
+    cast = torch.int8 if codes == "int8" else torch.float8_e4m3fn
+
+    def ri(lo, hi, *shape):
+        return torch.randint(lo, hi + 1, shape, generator=gen, device=cuda).float()
+
+    a, b = ri(-hi, hi, m, k).to(cast), ri(-hi_b, hi_b, n, k).to(cast)
+    kt, nt = -(-k // bk), -(-n // bn)
+    a_s, b_s = torch.exp2(ri(-1, 0, m, kt)), torch.exp2(ri(-1, 0, nt, kt))
+    bias, res = ri(-8, 8, n).bfloat16(), ri(-8, 8, m, n).bfloat16()
+    op = (tob.w8a8_block_int8_matmul_bias_act if codes == "int8"
+          else tob.w8a8_block_fp8_matmul_bias_act)
+    y = op(a, b, a_s, b_s, [bn, bk], bias, act="relu", residual=res, output_dtype=torch.bfloat16)
+    want = w8a8_exact(a, b, a_s, b_s, bn, bk, bias, "relu", res).bfloat16()
+    assert torch.equal(y, want)
+    y = op(a, b, a_s, b_s, [bn, bk], output_dtype=torch.float16)
+    assert torch.equal(y, w8a8_exact(a, b, a_s, b_s, bn, bk, None, None, None).half())

@@ -6,6 +6,9 @@ namespace tob {
 namespace sm100 {
 int linear_nt_launch(int kind, bool block_scaled, const void* x, int64_t ldx, const void* w,
                      int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st);
+// TO_EUNSUPPORTED (nothing launched) where the tiles do not apply.
+int linear_pair_launch(int kind, bool block_scaled, const void* a, int64_t lda, const void* b,
+                       int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st);
 }
 int linear_dense_simt_launch(const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
                              int64_t K, const LinEpi& ep, cudaStream_t st);
@@ -13,6 +16,14 @@ int linear_w8a8_simt_launch(bool fp8, const void* a, const void* b, int64_t M, i
                             int64_t bn, int64_t bk, const LinEpi& ep, cudaStream_t st);
 
 namespace {
+
+// Many tokens: CTA-pair tiles; few tokens, a small grid or any misalignment: weights as rows.
+int tensor_core_launch(int kind, bool block_scaled, const void* a, int64_t lda, const void* b,
+                       int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st) {
+  const int rc = sm100::linear_pair_launch(kind, block_scaled, a, lda, b, M, N, K, ep, st);
+  if (rc != TO_EUNSUPPORTED) return rc;
+  return sm100::linear_nt_launch(kind, block_scaled, a, lda, b, M, N, K, ep, st);
+}
 
 // Fills the epilogue common to both products; TO_OK or a recorded failure.
 int make_epi(LinEpi* ep, const char* op, const void* bias, int act, const void* res, int64_t ldr,
@@ -60,7 +71,7 @@ int w8a8_epi_entry(bool fp8, const void* a, const void* b, const float* a_s, con
   if (kt > 1 && bk % 128 != 0)
     return linear_w8a8_simt_launch(fp8, a, b, M, N, K, ep.bn, bk, ep, st);
   ep.kb_per_scale = kt > 1 ? (int)(bk / 128) : 1;
-  return sm100::linear_nt_launch(fp8 ? TO_E4M3 : TO_I8, kt > 1, a, K, b, M, N, K, ep, st);
+  return tensor_core_launch(fp8 ? TO_E4M3 : TO_I8, kt > 1, a, K, b, M, N, K, ep, st);
 }
 
 }  // namespace
@@ -87,7 +98,7 @@ int to_gemm_bias_act(const void* a, int64_t lda, const void* b, const void* bias
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == TO_F32 || K == 0)
     return linear_dense_simt_launch(a, lda, b, M, N, K, ep, st);
-  return sm100::linear_nt_launch(dtype, false, a, lda, b, M, N, K, ep, st);
+  return tensor_core_launch(dtype, false, a, lda, b, M, N, K, ep, st);
 }
 
 int to_w8a8_i8_gemm_bias_act(const int8_t* a, const int8_t* b, const float* a_s, const float* b_s,

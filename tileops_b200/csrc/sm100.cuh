@@ -96,6 +96,12 @@ __device__ __forceinline__ uint64_t policy_evict_last() {
   return p;
 }
 
+__device__ __forceinline__ uint64_t policy_evict_normal() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+
 // 2-D tiled load of box (x = inner coordinate in elements, y = row) into this CTA's shared
 // memory, completing `bytes` on `bar`. x must be a multiple of 16 bytes worth of elements.
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* m, int x, int y,
