@@ -27,7 +27,7 @@ __device__ __forceinline__ void store_out(void* c, int64_t idx, float v, const v
 template <typename T>
 __device__ __forceinline__ void finish_epi(const LinEpi& ep, int m, int n, float acc) {
   if (ep.bias != nullptr) acc += to_f32(reinterpret_cast<const T*>(ep.bias)[n]);
-  float v = epi_act<false>(acc, ep.act);
+  float v = epi_act_exact(acc, ep.act);
   if (ep.res != nullptr) v += to_f32(reinterpret_cast<const T*>(ep.res)[(int64_t)m * ep.ldr + n]);
   reinterpret_cast<T*>(ep.c)[(int64_t)m * ep.ldc + n] = from_f32<T>(v);
 }

@@ -7,8 +7,10 @@ namespace sm100 {
 int linear_nt_launch(int kind, bool block_scaled, const void* x, int64_t ldx, const void* w,
                      int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st);
 // TO_EUNSUPPORTED (nothing launched) where the tiles do not apply.
-int linear_pair_launch(int kind, bool block_scaled, const void* a, int64_t lda, const void* b,
-                       int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st);
+int linear_pair_launch(int kind, const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
+                       int64_t K, const LinEpi& ep, cudaStream_t st);
+int linear_bs_launch(int kind, const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
+                     int64_t K, const LinEpi& ep, cudaStream_t st);
 }
 int linear_dense_simt_launch(const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
                              int64_t K, const LinEpi& ep, cudaStream_t st);
@@ -17,10 +19,11 @@ int linear_w8a8_simt_launch(bool fp8, const void* a, const void* b, int64_t M, i
 
 namespace {
 
-// Many tokens: CTA-pair tiles; few tokens, a small grid or any misalignment: weights as rows.
+// Many tokens: CTA-pair tiles, or folding tiles with block scales; few tokens, a small grid or any misalignment: weights as rows.
 int tensor_core_launch(int kind, bool block_scaled, const void* a, int64_t lda, const void* b,
                        int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st) {
-  const int rc = sm100::linear_pair_launch(kind, block_scaled, a, lda, b, M, N, K, ep, st);
+  const int rc = block_scaled ? sm100::linear_bs_launch(kind, a, lda, b, M, N, K, ep, st)
+                              : sm100::linear_pair_launch(kind, a, lda, b, M, N, K, ep, st);
   if (rc != TO_EUNSUPPORTED) return rc;
   return sm100::linear_nt_launch(kind, block_scaled, a, lda, b, M, N, K, ep, st);
 }
@@ -44,6 +47,7 @@ int make_epi(LinEpi* ep, const char* op, const void* bias, int act, const void* 
   ep->ldc = ldc;
   ep->dtype = dtype;
   ep->act = act;
+  ep->form = act_form(act);
   return TO_OK;
 }
 

@@ -12,19 +12,38 @@ enum EpiAct : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3 };
 
 // Both gated forms are x * sigmoid(z): silu with z = x, gelu_tanh with z = 2 sqrt(2/pi)
 // (x + 0.044715 x^3), since (1 + tanh(u)) / 2 = sigmoid(2u). In this form nothing cancels for
-// negative x. FAST takes the hardware exponential and division (relative error about 1e-6 over
-// the range where the result is not negligible, far below half a step of a 16-bit result).
-template <bool FAST>
-__device__ __forceinline__ float x_sigmoid(float x, float z) {
-  if constexpr (FAST) return __fdividef(x, 1.0f + __expf(-z));
-  else return x / (1.0f + expf(-z));
-}
-template <bool FAST>
-__device__ __forceinline__ float epi_act(float x, int act) {
+// negative x.
+__device__ __forceinline__ float epi_act_exact(float x, int act) {
   if (act == kActNone) return x;
   if (act == kActRelu) return x < 0.0f ? 0.0f : x;  // NaN stays NaN
   const float z = act == kActSilu ? x : 1.5957691216057308f * fmaf(0.044715f * x * x, x, x);
-  return x_sigmoid<FAST>(x, z);
+  return x / (1.0f + expf(-z));
+}
+
+// The same for the tensor-core kernels, whose epilogues run once per tile: their time is the
+// fetching of their instructions (unrolled over 32 columns with a four-way choice each they took
+// 8000 cycles a chunk), so the four activations share two short forms chosen by numbers:
+//   plain  x < lo ? lo : x                           (none: lo = -inf, relu: 0)
+//   gated  x / (1 + 2^(x (c1 + c2 min(x^2, 1e30))))  (the exponent is -z log2(e))
+// with the hardware's exponential and division: a relative error of about 1e-6 where the result is
+// not negligible, far below half a step of a 16-bit result. The minimum keeps 0 * inf out of silu.
+struct ActForm {
+  int gated;
+  float lo, c1, c2;
+};
+inline ActForm act_form(int act) {
+  constexpr float kLog2e = 1.4426950408889634f, kGelu = 1.5957691216057308f;
+  if (act == kActSilu) return {1, 0.f, -kLog2e, 0.f};
+  if (act == kActGelu) return {1, 0.f, -kLog2e * kGelu, -kLog2e * kGelu * 0.044715f};
+  return {0, act == kActRelu ? 0.f : -__builtin_inff(), 0.f, 0.f};
+}
+__device__ __forceinline__ float act_plain(float x, const ActForm& f) {
+  return x < f.lo ? f.lo : x;  // NaN stays NaN
+}
+__device__ __forceinline__ float act_gated(float x, const ActForm& f) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * fmaf(f.c2, fminf(x * x, 1e30f), f.c1)));
+  return __fdividef(x, 1.0f + e);
 }
 
 // What a product's epilogue reads and writes besides the accumulators. Row strides in elements.
@@ -40,6 +59,7 @@ struct LinEpi {
   int64_t ldr = 0, ldc = 0;
   int dtype = TO_F32;
   int act = kActNone;
+  ActForm form = {};           // act_form(act)
 };
 
 // Element i of an array of `dtype` (TO_F32 / TO_F16 / TO_BF16) as fp32, and its store. The

@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
         const int s = it % ST;
         const uint32_t ph = (uint32_t)(it / ST) & 1u;
         const int k = (kb_lo + it) * C::kBK;
-        if (it >= ST && !mbar_wait(empty + s, ph ^ 1, abort_flag, err)) { ok = false; break; }
+        if (it >= ST && !mbar_wait_polled(empty + s, ph ^ 1, abort_flag, err)) { ok = false; break; }
         mbar_arrive_expect_tx(full + s, wts ? C::kWBytes : C::kXBytes);
         if (!wts) {
           tma_load_2d(sX + (size_t)s * C::kXBytes, &tmX, k, t0, full + s, pol);
@@ -209,10 +209,10 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
       bool any = false;
       for (int it = 0; it < kb_n; ++it) {
         const int s = it % ST;
-        if (!mbar_wait(full + s, (uint32_t)(it / ST) & 1u, abort_flag, err)) { ok = false; break; }
+        if (!mbar_wait_polled(full + s, (uint32_t)(it / ST) & 1u, abort_flag, err)) { ok = false; break; }
         const int b = BS ? it & 1 : 0;
         if (BS && it >= 2 &&
-            !mbar_wait(tempty + b, ((uint32_t)(it >> 1) & 1u) ^ 1, abort_flag, err)) {
+            !mbar_wait_polled(tempty + b, ((uint32_t)(it >> 1) & 1u) ^ 1, abort_flag, err)) {
           ok = false;
           break;
         }
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
                                 (int)min((int64_t)16, row_bytes - off), g.x_align, g.x, x_hi);
           }
         }
-        if (it >= ST && !mbar_wait(empty + s, ((uint32_t)(it / ST) & 1u) ^ 1, abort_flag, err)) {
+        if (it >= ST && !mbar_wait_polled(empty + s, ((uint32_t)(it / ST) & 1u) ^ 1, abort_flag, err)) {
           ok = false;
           break;
         }
@@ -309,12 +309,12 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
   const bool n_ok = n < g.N;
   const LinEpi& ep = g.ep;
   float* part = reinterpret_cast<float*>(smem_raw);  // [token][128] partial sums (ring reuse)
-  float bias = 0.f, sb = 1.f, sa_l[(C::kTpt + 31) / 32];
-  // One output value; every lane of the warp calls it (shuffled token scale).
-  auto finish = [&](float acc, float sa, int tok, float res) {
-    float v = BS ? acc : acc * (sa * sb);
-    v = epi_act<true>(v + bias, ep.act) + res;
-    if (n_ok) st_dtype(ep.c, (int64_t)(t0 + tok) * ep.ldc + n, ep.dtype, v);
+  float bias = 0.f, sb = 1.f;
+  // One output of token tok: acc is its scaled sum.
+  auto finish = [&](float acc, int tok, float res) {
+    const float v = acc + bias;
+    const float y = (ep.form.gated ? act_gated(v, ep.form) : act_plain(v, ep.form)) + res;
+    st_dtype(ep.c, (int64_t)(t0 + tok) * ep.ldc + n, ep.dtype, y);
   };
   if (epi && ok) {
     grid_dependency_wait();
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
     if (!BS && ep.b_s != nullptr && n_ok) sb = __ldg(ep.b_s + brow);
     const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * C::kTpt);
     if constexpr (BS) {
-      float run[C::kTpt];
+      float run[C::kTpt], sa_l[(C::kTpt + 31) / 32];
 #pragma unroll
       for (int j = 0; j < C::kTpt; ++j) run[j] = 0.f;
       for (int it = 0; it < kb_n; ++it) {
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
           sa_l[i] = t < tokens ? __ldg(ep.a_s + (int64_t)(t0 + t) * ep.a_s_ld + kb) : 0.f;
         }
         const int b = it & 1;
-        if (!mbar_wait(tfull + b, (uint32_t)(it >> 1) & 1u, abort_flag, err)) { ok = false; break; }
+        if (!mbar_wait_polled(tfull + b, (uint32_t)(it >> 1) & 1u, abort_flag, err)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < C::kTpt; c += 16) {
@@ -353,100 +353,76 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
         __syncwarp();
         if (lane == 0) mbar_arrive(tempty + b);
       }
+      // The ring is idle: the last tfull covers every MMA that read it.
       if (ok) {
-        if (S > 1) {
-          // The ring is idle only once every MMA of this CTA has read its operands: the last
-          // tfull covers them all.
 #pragma unroll
-          for (int j = 0; j < C::kTpt; ++j)
-            part[(half * C::kTpt + j) * 128 + q * 32 + lane] = run[j];
-        } else {
-#pragma unroll
-          for (int j = 0; j < C::kTpt; ++j) {
-            const int tok = half * C::kTpt + j;
-            if (tok >= tokens) break;
-            float res = 0.f;
-            if (ep.res != nullptr && n_ok)
-              res = ld_dtype(ep.res, (int64_t)(t0 + tok) * ep.ldr + n, ep.dtype);
-            finish(run[j], 1.f, tok, res);
-          }
-        }
+        for (int j = 0; j < C::kTpt; ++j)
+          part[(half * C::kTpt + j) * 128 + q * 32 + lane] = run[j];
       }
     } else {
-#pragma unroll
-      for (int i = 0; i < (C::kTpt + 31) / 32; ++i) {
-        const int t = half * C::kTpt + i * 32 + lane;
-        sa_l[i] = ep.a_s != nullptr && t < tokens ? __ldg(ep.a_s + (int64_t)(t0 + t) * ep.a_s_ld)
-                                                  : 1.f;
-      }
+      ok = mbar_wait_polled(tfull, 0, abort_flag, err);
+      tc_fence_after();
 #pragma unroll
       for (int c = 0; c < C::kTpt; c += 16) {
         const int tok0 = half * C::kTpt + c;
-        float res[16];
-        const bool direct = S == 1;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          res[j] = 0.f;
-          if (direct && ep.res != nullptr && n_ok && tok0 + j < tokens)
-            res[j] = ld_dtype(ep.res, (int64_t)(t0 + tok0 + j) * ep.ldr + n, ep.dtype);
-        }
-        if (c == 0) {
-          ok = mbar_wait(tfull, 0, abort_flag, err);
-          tc_fence_after();
-        }
-        if (!ok) break;
-        if (tok0 >= tokens) break;
+        if (!ok || tok0 >= tokens) break;
         uint32_t r[16];
         tmem_ld16(lane_addr + (uint32_t)c, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int tok = tok0 + j;
-          if (S > 1) {
-            reinterpret_cast<uint32_t*>(part)[tok * 128 + q * 32 + lane] = r[j];
-          } else {
-            const float sa = __shfl_sync(0xffffffffu, sa_l[(c + j) / 32], (c + j) & 31);
-            const float a = KD == Kind::I8 ? (float)(int32_t)r[j] : __uint_as_float(r[j]);
-            if (tok < tokens) finish(a, sa, tok, res[j]);
-          }
-        }
+        for (int j = 0; j < 16; ++j)
+          reinterpret_cast<uint32_t*>(part)[(tok0 + j) * 128 + q * 32 + lane] = r[j];
       }
     }
   }
-  if (S > 1) {
-    cluster_sync_all();  // every rank's partial sums are in its shared memory
-    if (epi && ok) {
-      // Rank r finishes tokens r, r + S, ...; the sums run over the ranks in order.
-      const uint32_t mine = smem_u32(part + q * 32 + lane);
-      for (int i = half; rank + i * S < tokens; i += C::kEpiWarps / 4) {
-        const int tok = rank + i * S;
-        float res = 0.f;
-        if (ep.res != nullptr && n_ok)
-          res = ld_dtype(ep.res, (int64_t)(t0 + tok) * ep.ldr + n, ep.dtype);
-        float sa = 1.f;
-        if (!BS && ep.a_s != nullptr) sa = __ldg(ep.a_s + (int64_t)(t0 + tok) * ep.a_s_ld);
-        uint32_t v[8];
+  // The sums go through shared memory, [token][128 columns], and a short loop over the tokens
+  // finishes them: this code runs once, so what it costs is the fetching of its instructions.
+  // Split K: rank r finishes tokens r, r + S, ..., each summed over the ranks in order. Otherwise
+  // every thread reads back its own tokens, so no barrier is needed.
+  if (S > 1) cluster_sync_all();
+  if (epi && ok && n_ok) {
+    const uint32_t mine = smem_u32(part + q * 32 + lane);
+    const int step = S > 1 ? S * (C::kEpiWarps / 4) : 1;
+    const int first = S > 1 ? rank + half * S : half * C::kTpt;
+    const int last = S > 1 ? tokens : min(tokens, (half + 1) * C::kTpt);
+    constexpr int U = 2;  // tokens whose loads are in flight together
+#pragma unroll 1
+    for (int tok = first; tok < last; tok += U * step) {
+      float res[U], sc[U];
+      uint32_t v[U][8];
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          v[s] = 0u;
-          if (s < S) {
-            const uint32_t addr = mapa_shared(mine + (uint32_t)tok * 512u, (uint32_t)s);
-            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v[s]) : "r"(addr) : "memory");
+      for (int u = 0; u < U; ++u) {
+        const int t = min(tok + u * step, last - 1);
+        if (S > 1) {
+#pragma unroll
+          for (int s = 0; s < 8; ++s) {
+            v[u][s] = 0u;
+            if (s < S)
+              asm volatile("ld.shared::cluster.u32 %0, [%1];"
+                           : "=r"(v[u][s])
+                           : "r"(mapa_shared(mine + (uint32_t)t * 512u, (uint32_t)s))
+                           : "memory");
+          }
+        } else {
+          v[u][0] = reinterpret_cast<const uint32_t*>(part)[t * 128 + q * 32 + lane];
+        }
+        res[u] = ep.res != nullptr ? ld_dtype(ep.res, (int64_t)(t0 + t) * ep.ldr + n, ep.dtype)
+                                   : 0.f;
+        sc[u] = 1.f;
+        if (!BS && ep.a_s != nullptr) sc[u] = __ldg(ep.a_s + (int64_t)(t0 + t) * ep.a_s_ld) * sb;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        uint32_t sum = v[u][0];
+        if (S > 1) {
+#pragma unroll
+          for (int s = 1; s < 8; ++s) {
+            if (KD == Kind::I8 && !BS) sum += v[u][s];
+            else if (s < S) sum = __float_as_uint(__uint_as_float(sum) + __uint_as_float(v[u][s]));
           }
         }
-        float acc;
-        if (KD == Kind::I8 && !BS) {
-          int32_t t = 0;
-#pragma unroll
-          for (int s = 0; s < 8; ++s) t += (int32_t)v[s];
-          acc = (float)t;
-        } else {
-          acc = __uint_as_float(v[0]);
-#pragma unroll
-          for (int s = 1; s < 8; ++s)
-            if (s < S) acc += __uint_as_float(v[s]);
-        }
-        finish(acc, sa, tok, res);
+        const float acc = KD == Kind::I8 && !BS ? (float)(int32_t)sum : __uint_as_float(sum);
+        if (tok + u * step < last) finish(acc * sc[u], tok + u * step, res[u]);
       }
     }
   }

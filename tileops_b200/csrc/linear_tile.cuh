@@ -1,0 +1,175 @@
+// Shared by the many-token kernels of the products with an epilogue (linear_pair_sm100.cu,
+// linear_bs_sm100.cu): tile order, the chunk that leaves through shared memory, tensor maps.
+#pragma once
+
+#include <cudaTypedefs.h>
+
+#include "linear_epi.cuh"
+#include "sm100.cuh"
+
+namespace tob {
+namespace sm100 {
+
+PFN_cuTensorMapEncodeTiled_v12000 get_encode();
+
+namespace {
+
+constexpr int kEpiWarpsT = 8;       // epilogue warps of a CTA, two per TMEM lane quarter
+constexpr int kSlab = 32 * 32 * 2;  // one 32 x 32 chunk of 16-bit results
+
+// Bands of M tiles, M fastest: the tiles in flight share a band's A rows and a few B columns.
+__device__ __forceinline__ void band_tile(int t, int m_tiles, int n_tiles, int band, int& mt,
+                                          int& nt) {
+  const int per = band * n_tiles;
+  const int b = t / per;
+  const int rows = min(band, m_tiles - b * band);
+  const int local = t - b * per;
+  mt = b * band + local % rows;
+  nt = local / rows;
+}
+
+__device__ __forceinline__ void epi_barrier() {  // the epilogue warps of this CTA
+  asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarpsT * 32) : "memory");
+}
+
+// Bias, activation, residual and store of one warp's 32 x 32 chunks. Two slabs of shared memory
+// alternate; a chunk's residual is copied into its slab one chunk ahead and overwritten there by
+// the result, which leaves by a TMA store. One mbarrier per slab, each used once per visit.
+struct ChunkWriter {
+  uint8_t* slab0;        // two slabs
+  uint64_t* rbar;        // two barriers
+  const CUtensorMap* tmC;
+  const CUtensorMap* tmR;
+  volatile int* abort_flag;
+  int* err;
+  ActForm form;
+  int dtype, lane;
+  bool res;
+  int cnt = 0;  // chunks visited: slab cnt & 1, residual phase (cnt >> 1) & 1
+
+  // The residual of the ahead-th chunk from now (0 or 1), at (col0, row0).
+  __device__ __forceinline__ void fetch(int ahead, int col0, int row0) {
+    if (!res || lane != 0) return;
+    bulk_wait_read<0>();  // no store still reads the slab
+    uint64_t* bar = rbar + ((cnt + ahead) & 1);
+    mbar_arrive_expect_tx(bar, kSlab);
+    tma_load_2d(slab0 + ((cnt + ahead) & 1) * kSlab, tmR, col0, row0, bar, policy_evict_first());
+  }
+  // Waits until the current chunk's slab may be written (with the residual in it).
+  __device__ __forceinline__ bool acquire() {
+    if (res) return mbar_wait_polled(rbar + (cnt & 1), (uint32_t)(cnt >> 1) & 1u, abort_flag, err);
+    if (lane == 0) bulk_wait_read<1>();  // the store before last has read this slab
+    __syncwarp();
+    return true;
+  }
+  // v: this lane's row of the chunk, scaled; bias: of its 32 columns, in shared memory. Straight
+  // code per step, one uniform choice around each (see ActForm).
+  __device__ __forceinline__ void put(float* v, const float* bias, int col0, int row0, bool store) {
+    uint8_t* slab = slab0 + (cnt & 1) * kSlab;
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      const float4 b = *reinterpret_cast<const float4*>(bias + i);
+      v[i] += b.x;
+      v[i + 1] += b.y;
+      v[i + 2] += b.z;
+      v[i + 3] += b.w;
+    }
+    if (form.gated) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = act_gated(v[i], form);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = act_plain(v[i], form);
+    }
+    // 16-byte pieces of 8 columns, swizzled as the TMA box is
+    auto at = [&](int c) {
+      return reinterpret_cast<uint4*>(slab + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4));
+    };
+    if (dtype == TO_BF16) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (res) w = *at(c);
+        uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const __nv_bfloat162 o =
+              __floats2bfloat162_rn(v[c * 8 + 2 * p] + __uint_as_float(wp[p] << 16),
+                                    v[c * 8 + 2 * p + 1] + __uint_as_float(wp[p] & 0xFFFF0000u));
+          wp[p] = *reinterpret_cast<const uint32_t*>(&o);
+        }
+        *at(c) = w;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (res) w = *at(c);
+        uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&wp[p]));
+          const __half2 o = __floats2half2_rn(v[c * 8 + 2 * p] + f.x, v[c * 8 + 2 * p + 1] + f.y);
+          wp[p] = *reinterpret_cast<const uint32_t*>(&o);
+        }
+        *at(c) = w;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && store) {
+      tma_store_2d(tmC, col0, row0, slab);
+      bulk_commit();
+    }
+    ++cnt;
+  }
+};
+
+// Tensor map with the given box and swizzle; strides in bytes.
+inline int tiled_map(CUtensorMap* out, CUtensorMapDataType dt, const void* p, int rank,
+              const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+              CUtensorMapSwizzle sw) {
+  auto encode = get_encode();
+  if (!encode) return fail(TO_ECUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = encode(out, dt, (cuuint32_t)rank, const_cast<void*>(p), dims, strides, box,
+                            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TO_OK
+                           : fail(TO_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+}
+
+// K-major operand: boxes of box_rows rows x `slices` 128-byte slices (3-D view, K whole slices), or
+// of one slice (2-D, slices = 1).
+inline int kmajor_map(CUtensorMap* out, const void* p, int64_t rows, int64_t K, int64_t pitch,
+                      int elem, int box_rows, int slices) {
+  const auto dt = elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  const cuuint32_t bk = (cuuint32_t)(128 / elem);
+  if (slices > 1) {
+    const cuuint64_t dims[3] = {bk, (cuuint64_t)rows, (cuuint64_t)(K / bk)};
+    const cuuint64_t strides[2] = {(cuuint64_t)pitch, 128};
+    const cuuint32_t box[3] = {bk, (cuuint32_t)box_rows, (cuuint32_t)slices};
+    return tiled_map(out, dt, p, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)pitch};
+  const cuuint32_t box[2] = {bk, (cuuint32_t)box_rows};
+  return tiled_map(out, dt, p, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// The map of a 16-bit [rows, cols] output or residual: 32 x 32 boxes, 64-byte swizzle.
+inline int chunk_map(CUtensorMap* out, const void* p, int64_t rows, int64_t cols, int64_t ld) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
+  const cuuint32_t box[2] = {32, 32};
+  return tiled_map(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, p, 2, dims, strides, box,
+                   CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+inline bool aligned_rows(const void* p, int64_t pitch) {
+  return ((reinterpret_cast<uint64_t>(p) | (uint64_t)pitch) & 15u) == 0;
+}
+
+}  // namespace
+}  // namespace sm100
+}  // namespace tob

@@ -80,6 +80,30 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// The same wait, polling a thousand times (some tens of microseconds) before it reads the global
+// timer, which costs hundreds of cycles: for waits that end in less than that.
+__device__ __forceinline__ bool mbar_wait_polled(uint64_t* bar, uint32_t parity,
+                                                 volatile int* abort, int* err) {
+#pragma unroll 1
+  for (int i = 0; i < 1024; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity, abort, err);
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+// mbar_wait_polled by a whole converged warp, which leaves it converged and of one mind.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                               int* err) {
+  return __all_sync(0xffffffffu, mbar_wait_polled(bar, parity, abort, err));
+}
+
 // ------------------------------------------------------------------ TMA
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
