@@ -279,6 +279,8 @@ __global__ void __launch_bounds__(kThreadsB, 1)
       while (mine < c_count && n0 + (c_first + mine) * 32 < g.N) ++mine;
       if (row0 >= g.M) mine = 0;
       if (mine > 0) wr.fetch(0, n0 + c_first * 32, row0);
+      if (mine > 1) wr.fetch(1, n0 + c_first * 32 + 32, row0);
+      for (int j = 2; j < mine; ++j) wr.want(n0 + (c_first + j) * 32, row0);
 
       float run[kMax * 32];
 #pragma unroll
@@ -338,9 +340,9 @@ __global__ void __launch_bounds__(kThreadsB, 1)
 #pragma unroll 1
       for (int j = 0; j < mine; ++j) {
         const int c0 = (c_first + j) * 32;
-        if (j + 1 < mine) wr.fetch(1, n0 + c0 + 32, row0);
         if (!wr.acquire()) ok = false;
         wr.put(run, bias + c0, n0 + c0, row0, ok);
+        if (j + 2 < mine) wr.fetch(1, n0 + c0 + 64, row0);
 #pragma unroll
         for (int i = 0; i < (kMax - 1) * 32; ++i) run[i] = run[i + 32];
       }

@@ -197,49 +197,55 @@ __global__ void __launch_bounds__(kThreadsP, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader only)
-    if (lane == 0 && rank == 0) {
+    // The whole warp walks the loop and one lane issues: addresses and descriptors then stay in
+    // uniform registers.
+    if (rank == 0) {
       constexpr uint32_t idesc =
           make_idesc_major(Tr::kDFmt, Tr::kAFmt, Tr::kBFmt, 256, BN, 0, C::kMn ? 1 : 0);
-      bool ok = true, any = false;
-      int it = 0, fill = 0;  // stages consumed; accumulator fills started
+      const uint64_t adesc = smem_desc_kmajor_sw128(smem_u32(sA));
+      const uint64_t bdesc = C::kMn ? smem_desc_mnmajor_sw128(smem_u32(sB), 16384, 1024)
+                                    : smem_desc_kmajor_sw128(smem_u32(sB));
+      const bool issue = elect_one();
+      bool ok = true;
+      int fill = 0, s = 0;  // accumulator fills started; stage
+      uint32_t ph = 0;
       for (int t = pair; ok && t < tiles; t += pairs) {
-        if (fill >= 2 &&
-            !mbar_wait_polled(tempty + (fill & 1), ((uint32_t)(fill >> 1) & 1u) ^ 1, abort_flag, err)) {
-          ok = false;
-          break;
-        }
-        const uint32_t d = tmem + (uint32_t)((fill & 1) * BN);
-        for (int st = 0; st < steps; ++st, ++it) {
-          const int s = it % ST;
-          if (!mbar_wait_polled(full + s, (uint32_t)(it / ST) & 1u, abort_flag, err)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t a0 = smem_u32(sA + (size_t)s * C::kABytes);
-          const uint32_t b0 = smem_u32(sB + (size_t)s * C::kBBytes);
-#pragma unroll
-          for (int c = 0; c < kKC; ++c) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint64_t bd =
-                  C::kMn ? smem_desc_mnmajor_sw128(b0 + c * 8192 + 2048 * k, 16384, 1024)
-                         : smem_desc_kmajor_sw128(b0 + c * C::kBCh + 32 * k);
-              umma_pair<KD>(d, smem_desc_kmajor_sw128(a0 + c * C::kACh + 32 * k), bd, idesc,
-                            (st | c | k) != 0);
-            }
-          }
-          any = true;
-          umma_commit_pair_mc(empty + s, 0x3);
-        }
+        if (fill >= 2)
+          ok = mbar_wait_warp(tempty + (fill & 1), ((uint32_t)(fill >> 1) & 1u) ^ 1, abort_flag,
+                              err);
         if (!ok) break;
-        umma_commit_pair_mc(tfull + (fill & 1), 0x3);
+        const uint32_t d = tmem + (uint32_t)((fill & 1) * BN);
+        for (int st = 0; st < steps; ++st) {
+          ok = mbar_wait_warp(full + s, ph, abort_flag, err);
+          if (!ok) break;
+          tc_fence_after();
+          if (issue) {
+            const uint64_t ad = adesc + (uint64_t)(s * (C::kABytes >> 4));
+            const uint64_t bd = bdesc + (uint64_t)(s * (C::kBBytes >> 4));
+#pragma unroll
+            for (int i = 0; i < 4 * kKC; ++i) {
+              // 32 bytes of K: within a slice 32 B on, MN-major 16 K rows (2 KB) on
+              const int ao = (i / 4) * C::kACh + 32 * (i % 4);
+              const int bo = C::kMn ? (i / 4) * 8192 + 2048 * (i % 4)
+                                    : (i / 4) * C::kBCh + 32 * (i % 4);
+              umma_pair<KD>(d, ad + (ao >> 4), bd + (bo >> 4), idesc, (st | i) != 0);
+            }
+            umma_commit_pair_mc(empty + s, 0x3);
+            if (st == steps - 1) umma_commit_pair_mc(tfull + (fill & 1), 0x3);
+          }
+          __syncwarp();
+          if (++s == ST) { s = 0; ph ^= 1; }
+        }
         ++fill;
       }
-      if (!ok && any) {
+      if (!ok && issue) {
         // Unwinding: wait (bounded) until the MMAs already issued have finished.
         umma_commit_pair(drain);
         const uint64_t tw = globaltimer_ns();
         while (!mbar_try_wait(drain, 0) && globaltimer_ns() - tw < kWaitLimitNs) {
         }
       }
+      __syncwarp();
     }
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
@@ -277,6 +283,8 @@ __global__ void __launch_bounds__(kThreadsP, 1)
       // After a failed wait a warp still walks the tiles: the others count on it at the barriers.
       if (!ok) continue;
       if (mine > 0) wr.fetch(0, n0 + chunk_col(0), row0);
+      if (mine > 1) wr.fetch(1, n0 + chunk_col(1), row0);
+      for (int j = 2; j < mine; ++j) wr.want(n0 + chunk_col(j), row0);
       const float sa = ep.a_s != nullptr ? __ldg(ep.a_s + (int64_t)row * ep.a_s_ld) : 1.f;
       const int b = fill & 1;
       if (!mbar_wait_polled(tfull + b, (uint32_t)(fill >> 1) & 1u, abort_flag, err)) {
@@ -304,9 +312,9 @@ __global__ void __launch_bounds__(kThreadsP, 1)
             v[i + u] = C::kMn ? a : a * (sa * sbv[u]);
           }
         }
-        if (j + 1 < mine) wr.fetch(1, n0 + chunk_col(j + 1), row0);
         if (!wr.acquire()) ok = false;
         wr.put(v, bias + c0, n0 + c0, row0, ok);
+        if (j + 2 < mine) wr.fetch(1, n0 + chunk_col(j + 2), row0);
       }
       tc_fence_before();
       __syncwarp();

@@ -33,8 +33,10 @@ __device__ __forceinline__ void epi_barrier() {  // the epilogue warps of this C
 }
 
 // Bias, activation, residual and store of one warp's 32 x 32 chunks. Two slabs of shared memory
-// alternate; a chunk's residual is copied into its slab one chunk ahead and overwritten there by
-// the result, which leaves by a TMA store. One mbarrier per slab, each used once per visit.
+// alternate; a chunk's residual is copied into its slab up to two chunks ahead and overwritten there
+// by the result, which leaves by a TMA store. One mbarrier per slab, each used once per visit.
+// Order per tile: fetch(0), fetch(1); then per chunk acquire, put and, after it, fetch(1) for the
+// chunk after next. want() brings the residual of later chunks near (into L2) at the tile's start.
 struct ChunkWriter {
   uint8_t* slab0;        // two slabs
   uint64_t* rbar;        // two barriers
@@ -47,6 +49,13 @@ struct ChunkWriter {
   bool res;
   int cnt = 0;  // chunks visited: slab cnt & 1, residual phase (cnt >> 1) & 1
 
+  __device__ __forceinline__ void want(int col0, int row0) {
+    if (!res || lane != 0) return;
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
+                     reinterpret_cast<uint64_t>(tmR)),
+                 "r"(col0), "r"(row0)
+                 : "memory");
+  }
   // The residual of the ahead-th chunk from now (0 or 1), at (col0, row0).
   __device__ __forceinline__ void fetch(int ahead, int col0, int row0) {
     if (!res || lane != 0) return;
