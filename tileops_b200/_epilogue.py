@@ -1,5 +1,8 @@
 """Argument checks shared by the products with bias, activation and residual in their epilogue
-(``gemm_bias_act``, ``w8a8_block_int8_matmul_bias_act``, ``w8a8_block_fp8_matmul_bias_act``)."""
+(``gemm_bias_act``, ``w8a8_block_int8_matmul_bias_act``, ``w8a8_block_fp8_matmul_bias_act``).
+
+A decode step makes several such calls per layer on kernels of a few microseconds, so the common
+case (contiguous operands) does nothing but compare."""
 
 from __future__ import annotations
 
@@ -12,45 +15,54 @@ from .fused import _row_stride
 ACT_CODES = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
+def _same(op: str, name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device) -> None:
+    if t.dtype != dtype:
+        raise TypeError(f"{op}: {name}.dtype={t.dtype} != output dtype {dtype}")
+    if t.device != device:
+        raise TypeError(f"{op}: all tensors must be on {device} ({name} is on {t.device})")
+
+
 def check(op: str, shape: tuple, n: int, dtype: torch.dtype, device: torch.device,
           bias: Optional[torch.Tensor], act: Optional[str], residual: Optional[torch.Tensor],
           out: Optional[torch.Tensor]) -> int:
     """Checks the epilogue's operands against an output of ``shape`` (last dimension ``n``) and
     returns the activation's code. Raised before any device work."""
-    if act not in ACT_CODES:
+    code = ACT_CODES.get(act) if act is None or isinstance(act, str) else None
+    if code is None:
         raise ValueError(f"{op}: act must be None, 'relu', 'silu' or 'gelu' (got {act!r})")
-    if bias is not None and tuple(bias.shape) != (n,):
+    if bias is not None and bias.shape != (n,):
         raise ValueError(f"{op}: bias.shape={tuple(bias.shape)} != ({n},)")
-    for name, t in (("residual", residual), ("out", out)):
-        if t is not None and tuple(t.shape) != tuple(shape):
-            raise ValueError(f"{op}: {name}.shape={tuple(t.shape)} != {tuple(shape)}")
-    for name, t in (("bias", bias), ("residual", residual), ("out", out)):
-        if t is None:
-            continue
-        if t.dtype != dtype:
-            raise TypeError(f"{op}: {name}.dtype={t.dtype} != output dtype {dtype}")
-        if t.device != device:
-            raise TypeError(f"{op}: all tensors must be on {device} ({name} is on {t.device})")
-    return ACT_CODES[act]
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"{op}: residual.shape={tuple(residual.shape)} != {tuple(shape)}")
+    if out is not None and out.shape != shape:
+        raise ValueError(f"{op}: out.shape={tuple(out.shape)} != {tuple(shape)}")
+    if bias is not None:
+        _same(op, "bias", bias, dtype, device)
+    if residual is not None:
+        _same(op, "residual", residual, dtype, device)
+    if out is not None:
+        _same(op, "out", out, dtype, device)
+    return code
 
 
-def prepare(shape: tuple, n: int, dtype: torch.dtype, device: torch.device,
+def prepare(shape: tuple, n: int, like: torch.Tensor, dtype: torch.dtype,
             bias: Optional[torch.Tensor], residual: Optional[torch.Tensor],
             out: Optional[torch.Tensor]):
     """``(bias, residual, ldr, dst, ldc)``: the tensors the kernel reads and writes, rows strided
     as they are where their last dimension is contiguous, copied otherwise. ``dst`` is ``out`` or,
     where the kernel cannot write that in place, a fresh tensor to copy into it (finish)."""
-    if bias is not None and n > 1 and bias.stride(0) != 1:
+    if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    ldr = 0
-    if residual is not None:
+    ldr = n
+    if residual is not None and not residual.is_contiguous():
         ldr = _row_stride(residual)
         if ldr is None:
             residual, ldr = residual.contiguous(), n
-    ldc = None if out is None else _row_stride(out)
-    if ldc is None:
-        return bias, residual, ldr, torch.empty(shape, dtype=dtype, device=device), n
-    return bias, residual, ldr, out, ldc
+    if out is not None:
+        ldc = n if out.is_contiguous() else _row_stride(out)
+        if ldc is not None:
+            return bias, residual, ldr, out, ldc
+    return bias, residual, ldr, like.new_empty(shape, dtype=dtype), n
 
 
 def finish(dst: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:

@@ -80,12 +80,14 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
     code = _epilogue.check(op, (m, n), n, dtype, device, bias, act, residual, out)
     idx = _lib.ensure_device(a, op)
     _lib.same_device(op, a, b)
-    lda = _row_stride(a)
-    if lda is None:
-        a, lda = a.contiguous(), k
+    lda = k
+    if not a.is_contiguous():
+        lda = _row_stride(a)
+        if lda is None:
+            a, lda = a.contiguous(), k
     if not b.is_contiguous():
         b = b.contiguous()
-    bias, residual, ldr, dst, ldc = _epilogue.prepare((m, n), n, dtype, device, bias, residual, out)
+    bias, residual, ldr, dst, ldc = _epilogue.prepare((m, n), n, a, dtype, bias, residual, out)
     _lib.call("to_gemm_bias_act", a.data_ptr(), lda, b.data_ptr(), _lib.ptr(bias), code,
               _lib.ptr(residual), ldr, dst.data_ptr(), ldc, _lib.DTYPE_CODES[dtype], m, n, k,
               _lib.stream_ptr(idx))

@@ -149,6 +149,14 @@ def act_and_mul_group_quant(a: torch.Tensor, b: torch.Tensor, group_size: int, *
     return q, s
 
 
+def _check_like(op: str, name: str, t: torch.Tensor, dtype: torch.dtype,
+                device: torch.device) -> None:
+    if t.dtype != dtype:
+        raise TypeError(f"{op}: {name}.dtype={t.dtype} != x.dtype={dtype}")
+    if t.device != device:
+        raise TypeError(f"{op}: all tensors must be on {device} ({name} is on {t.device})")
+
+
 def add_rms_norm_group_quant(x: torch.Tensor, weight: torch.Tensor, group_size: int,
                              residual: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
                              dtype: Optional[torch.dtype] = None, quant_eps: float = 1e-10,
@@ -171,59 +179,68 @@ def add_rms_norm_group_quant(x: torch.Tensor, weight: torch.Tensor, group_size: 
     a NaN has NaN scales, e4m3 NaN codes and int8 zeros; a row of zeros has codes 0 and scales
     quant_eps / qmax."""
     op = "add_rms_norm_group_quant"
-    if x.dim() == 0 or tuple(weight.shape) != (x.shape[-1],):
+    if x.dim() == 0 or weight.shape != x.shape[-1:]:
         raise ValueError(f"{op}: weight.shape={tuple(weight.shape)} does not match the last "
                          f"dimension of x {tuple(x.shape)}")
     cols = x.shape[-1]
     if group_size <= 0 or cols % group_size != 0:
         raise ValueError(f"{op}: the last dimension of `x` {cols} must be divisible by "
                          f"`group_size` {group_size}")
-    dtype = torch.float8_e4m3fn if dtype is None else dtype
-    if dtype not in (torch.float8_e4m3fn, torch.int8):
-        raise TypeError(f"{op}: codes must be torch.float8_e4m3fn or torch.int8 (got {dtype})")
-    if dtype == torch.int8 and (use_ue8m0 or column_major_scales):
-        raise ValueError(f"{op}: use_ue8m0 and column_major_scales are FP8 options")
+    if dtype is None:
+        dtype = torch.float8_e4m3fn
+    code = 4 if dtype == torch.float8_e4m3fn else 3
+    if code == 3:
+        if dtype != torch.int8:
+            raise TypeError(f"{op}: codes must be torch.float8_e4m3fn or torch.int8 (got {dtype})")
+        if use_ue8m0 or column_major_scales:
+            raise ValueError(f"{op}: use_ue8m0 and column_major_scales are FP8 options")
     if column_major_scales and x.dim() != 2:
         raise ValueError(f"{op}: column_major_scales needs a 2-D input")
-    if residual_out is not None and residual is None:
-        raise ValueError(f"{op}: residual_out needs a residual")
-    xd = x.dtype
-    for name, t in (("weight", weight), ("residual", residual), ("residual_out", residual_out)):
-        if t is None:
-            continue
-        if name != "weight" and t.shape != x.shape:
-            raise ValueError(f"{op}: {name}.shape={tuple(t.shape)} != x.shape={tuple(x.shape)}")
-        if t.dtype != xd:
-            raise TypeError(f"{op}: {name}.dtype={t.dtype} != x.dtype={xd}")
-        if t.device != x.device:
-            raise TypeError(f"{op}: all tensors must be on {x.device} ({name} is on {t.device})")
+    xd, device = x.dtype, x.device
+    _check_like(op, "weight", weight, xd, device)
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"{op}: residual.shape={tuple(residual.shape)} != "
+                             f"x.shape={tuple(x.shape)}")
+        _check_like(op, "residual", residual, xd, device)
+    if residual_out is not None:
+        if residual is None:
+            raise ValueError(f"{op}: residual_out needs a residual")
+        if residual_out.shape != x.shape:
+            raise ValueError(f"{op}: residual_out.shape={tuple(residual_out.shape)} != "
+                             f"x.shape={tuple(x.shape)}")
+        _check_like(op, "residual_out", residual_out, xd, device)
     idx = _lib.ensure_device(x, op)
     if xd not in _DTYPES:
         raise TypeError(f"{op}: unsupported dtype {xd} (float32, float16 and bfloat16 are "
                         "supported)")
+    lead = x.shape[:-1]
     rows = x.numel() // cols if cols else 0
-    ldx = _row_stride(x)
-    ldr = ldh = 0
+    ldx = ldr = ldh = cols
+    if not x.is_contiguous():
+        ldx = _row_stride(x)
+        if ldx is None:
+            x, ldx = x.contiguous(), cols
+    q = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
     dst = None
     if residual is not None:
-        ldr = _row_stride(residual)
-        ldh = None if residual_out is None else _row_stride(residual_out)
-        if ldh is None:
-            dst, ldh = torch.empty(x.shape, dtype=xd, device=x.device), cols
+        if not residual.is_contiguous():
+            ldr = _row_stride(residual)
+            if ldr is None:
+                residual, ldr = residual.contiguous(), cols
+        if residual_out is not None:
+            ldh = cols if residual_out.is_contiguous() else _row_stride(residual_out)
+        if residual_out is None or ldh is None:
+            dst, ldh = torch.empty_like(x, memory_format=torch.contiguous_format), cols
         else:
             dst = residual_out
-        if ldr is None:
-            residual, ldr = residual.contiguous(), cols
-    if ldx is None:
-        x, ldx = x.contiguous(), cols
     if not weight.is_contiguous():
         weight = weight.contiguous()
-    q = torch.empty(x.shape, dtype=dtype, device=x.device)
-    s = torch.empty(*x.shape[:-1], cols // group_size, dtype=torch.float32, device=x.device)
+    s = x.new_empty((*lead, cols // group_size), dtype=torch.float32)
     _lib.call("to_add_rms_norm_group_quant", x.data_ptr(), ldx, _lib.ptr(residual), ldr,
               weight.data_ptr(), _lib.DTYPE_CODES[xd], rows, cols, group_size, eps, quant_eps,
-              1 if use_ue8m0 else 0, 1 if column_major_scales else 0, _lib.DTYPE_CODES[dtype],
-              q.data_ptr(), s.data_ptr(), _lib.ptr(dst), ldh, _lib.stream_ptr(idx))
+              1 if use_ue8m0 else 0, 1 if column_major_scales else 0, code, q.data_ptr(),
+              s.data_ptr(), _lib.ptr(dst), ldh, _lib.stream_ptr(idx))
     if residual is None:
         return q, s
     if residual_out is not None and dst is not residual_out:

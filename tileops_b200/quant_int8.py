@@ -245,8 +245,8 @@ def _run_w8a8_bias_act(entry, op, a, b, a_s, b_s, block_n, block_k, m, n, k, bia
         a_s = a_s.to(torch.float32).contiguous()
     if b_s.dtype != torch.float32 or not b_s.is_contiguous():
         b_s = b_s.to(torch.float32).contiguous()
-    bias, residual, ldr, dst, ldc = _epilogue.prepare(shape, n, output_dtype, device, bias,
-                                                      residual, out)
+    bias, residual, ldr, dst, ldc = _epilogue.prepare(shape, n, a, output_dtype, bias, residual,
+                                                      out)
     _lib.call(entry, a.data_ptr(), b.data_ptr(), a_s.data_ptr(), b_s.data_ptr(), _lib.ptr(bias),
               code, _lib.ptr(residual), ldr, dst.data_ptr(), ldc,
               _lib.DTYPE_CODES[output_dtype], m, n, k, block_n, block_k, _lib.stream_ptr(idx))
