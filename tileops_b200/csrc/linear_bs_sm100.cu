@@ -136,6 +136,8 @@ __global__ void __launch_bounds__(kThreadsB, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
 
+  if (threadIdx.x == 0) grid_dependents_launch();  // the next kernel may set itself up
+
   if (warp < kEpi0B) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (misaligned) {
@@ -145,7 +147,7 @@ __global__ void __launch_bounds__(kThreadsB, 1)
       if (lane == 0) {
         const bool is_a = warp == 0;
         const uint64_t pol = policy_evict_normal();
-        if (is_a) grid_dependency_wait();  // A may be the previous kernel's output
+        if (is_a || !ep.early_weights) grid_dependency_wait();
         uint32_t issued_mask = 0, issued_phase = 0;
         bool ok = true;
         int it = 0;
@@ -165,9 +167,7 @@ __global__ void __launch_bounds__(kThreadsB, 1)
             issued_phase = (issued_phase & ~(1u << s)) | (ph << s);
           }
         }
-        if (ok) {
-          if (is_a) grid_dependents_launch();
-        } else {
+        if (!ok) {
           // Unwinding: let the copies in flight land (one deadline for all stages).
           const uint64_t tw = globaltimer_ns();
           for (int i = 0; i < ST; ++i)
@@ -356,6 +356,7 @@ __global__ void __launch_bounds__(kThreadsB, 1)
     }
   }
 
+  grid_dependency_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -393,12 +394,10 @@ int launch_bs(const void* a, int64_t lda, const void* b, int64_t M, int64_t N, i
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  if (launch_overlap()) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 1;
-  }
+  cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, tc, tr, g, device_error_ptr());
   if (e != cudaSuccess) return cuda_fail(e, "linear epilogue (block scales) launch");
   return check_launch("linear epilogue (block scales)");

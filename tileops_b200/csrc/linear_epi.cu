@@ -48,6 +48,7 @@ int make_epi(LinEpi* ep, const char* op, const void* bias, int act, const void* 
   ep->dtype = dtype;
   ep->act = act;
   ep->form = act_form(act);
+  ep->early_weights = launch_overlap();
   return TO_OK;
 }
 

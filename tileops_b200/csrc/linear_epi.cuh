@@ -46,6 +46,13 @@ __device__ __forceinline__ float act_gated(float x, const ActForm& f) {
   return __fdividef(x, 1.0f + e);
 }
 
+// Launches of these kernels carry the programmatic-dependency attribute always: a kernel's blocks may
+// start (barriers, tensor memory, tensor maps) while the previous kernel of the stream drains, and
+// every thread that touches global memory first waits for that kernel's completion
+// (griddepcontrol.wait), so the order of the stream holds as with plain launches. Only with launch
+// overlap switched on (to_set_launch_overlap) do the weights' copies skip that wait. Each block
+// waits before it ends, so completion stays transitive along a chain.
+
 // What a product's epilogue reads and writes besides the accumulators. Row strides in elements.
 struct LinEpi {
   const float* a_s = nullptr;  // scale of token m in K block kb: a_s[m * a_s_ld + kb]; null: 1
@@ -59,6 +66,7 @@ struct LinEpi {
   int64_t ldr = 0, ldc = 0;
   int dtype = TO_F32;
   int act = kActNone;
+  int early_weights = 0;       // launch overlap: weights are read before the previous kernel ends
   ActForm form = {};           // act_form(act)
 };
 

@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   bool ok = !misaligned;
+  if (threadIdx.x == 0) grid_dependents_launch();  // the next kernel may set itself up
 
   if (!ok) {
     // nothing to do; fall through to the barriers and the teardown
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
       const bool wts = warp == 0;
       // The weights stream once past L2's other contents; every column tile re-reads the tokens.
       const uint64_t pol = wts ? policy_evict_first() : policy_evict_last();
-      if (!wts) grid_dependency_wait();  // the tokens may be the previous kernel's output
+      if (!wts || !g.ep.early_weights) grid_dependency_wait();
       uint32_t issued_mask = 0, issued_phase = 0;
       for (int it = 0; it < kb_n; ++it) {
         const int s = it % ST;
@@ -189,9 +190,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
         issued_mask |= 1u << s;
         issued_phase = (issued_phase & ~(1u << s)) | (ph << s);
       }
-      if (ok) {
-        if (wts) grid_dependents_launch();
-      } else {
+      if (!ok) {
         // Unwinding: let the copies in flight land before the CTA exits (one deadline).
         const uint64_t tw = globaltimer_ns();
         for (int i = 0; i < ST; ++i)
@@ -426,6 +425,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
       }
     }
   }
+  grid_dependency_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -530,13 +530,10 @@ int launch_nt(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, i
   attr[0].val.clusterDim.x = (unsigned)S;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (launch_overlap()) {
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 2;
-  }
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, tx, g, device_error_ptr());
   if (e != cudaSuccess) return cuda_fail(e, "linear epilogue launch");
   return check_launch("linear epilogue");

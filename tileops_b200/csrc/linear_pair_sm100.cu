@@ -118,6 +118,8 @@ __global__ void __launch_bounds__(kThreadsP, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
 
+  if (threadIdx.x == 0) grid_dependents_launch();  // the next kernel may set itself up
+
   if (misaligned) {
     // nothing to do; fall through to the teardown
   } else if (warp == 0 || warp == kBWarpP) {
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(kThreadsP, 1)
                            : is_a     ? policy_evict_last()
                                       : policy_evict_first();
       const uint32_t lead_full = mapa_shared(smem_u32(full), 0);
-      if (is_a) grid_dependency_wait();  // A may be the previous kernel's output
+      if (is_a || !ep.early_weights) grid_dependency_wait();
       uint32_t issued_mask = 0, issued_phase = 0;
       bool ok = true;
       int it = 0;  // stages issued
@@ -178,7 +180,6 @@ __global__ void __launch_bounds__(kThreadsP, 1)
           }
         }
       }
-      if (ok && is_a) grid_dependents_launch();
       if (!ok && rank == 0 && is_a) {
         // Unwinding: the leader's full barriers count both CTAs' bytes; let them land. One
         // deadline for all stages: a stage whose other copies were never issued cannot complete.
@@ -330,6 +331,7 @@ __global__ void __launch_bounds__(kThreadsP, 1)
     }
   }
 
+  grid_dependency_wait();
   tc_fence_before();
   cluster_sync_all();  // both epilogues are done with TMEM; no signal to a peer is pending
   if (warp == 1) {
@@ -391,13 +393,10 @@ int launch_pair(const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (launch_overlap()) {
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 2;
-  }
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, tc, tr, g, device_error_ptr());
   if (e != cudaSuccess) return cuda_fail(e, "linear epilogue (pairs) launch");
   return check_launch("linear epilogue (pairs)");

@@ -55,6 +55,10 @@ __global__ void __launch_bounds__(1024) k_norm_quant(const NormArgs a) {
   __shared__ float red_sum[32];
   __shared__ unsigned red_max[32];
   extern __shared__ unsigned gmax[];  // kGroupShared: [rows of the CTA][groups]
+  // Launched as a programmatic dependent: blocks may start while the previous kernel drains, and
+  // wait for its completion before they touch memory.
+  grid_dependents_launch();
+  grid_dependency_wait();
   const int team = a.team;
   const int tid = (int)threadIdx.x % team, local = (int)threadIdx.x / team;
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x / team) + local;
@@ -263,8 +267,18 @@ int launch_norm(NormArgs a, cudaStream_t st) {
   }
   const int64_t blocks = ceil_div(a.rows, per_cta);
   if (blocks > INT32_MAX) return fail(TO_EUNSUPPORTED, "add_rms_norm_group_quant: too many rows");
-  k_norm_quant<T, Q, V, MAXV, MODE>
-      <<<(unsigned)blocks, (unsigned)(team * per_cta), smem, st>>>(a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+  cfg.blockDim = dim3((unsigned)(team * per_cta), 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_norm_quant<T, Q, V, MAXV, MODE>, a);
+  if (e != cudaSuccess) return cuda_fail(e, "add_rms_norm_group_quant launch");
   return check_launch("add_rms_norm_group_quant");
 }
 
