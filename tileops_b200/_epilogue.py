@@ -15,11 +15,10 @@ from .fused import _row_stride
 ACT_CODES = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
-def _same(op: str, name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device) -> None:
+def _refuse(op: str, name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device) -> None:
     if t.dtype != dtype:
         raise TypeError(f"{op}: {name}.dtype={t.dtype} != output dtype {dtype}")
-    if t.device != device:
-        raise TypeError(f"{op}: all tensors must be on {device} ({name} is on {t.device})")
+    raise TypeError(f"{op}: all tensors must be on {device} ({name} is on {t.device})")
 
 
 def check(op: str, shape: tuple, n: int, dtype: torch.dtype, device: torch.device,
@@ -27,7 +26,10 @@ def check(op: str, shape: tuple, n: int, dtype: torch.dtype, device: torch.devic
           out: Optional[torch.Tensor]) -> int:
     """Checks the epilogue's operands against an output of ``shape`` (last dimension ``n``) and
     returns the activation's code. Raised before any device work."""
-    code = ACT_CODES.get(act) if act is None or isinstance(act, str) else None
+    try:
+        code = ACT_CODES[act]
+    except (KeyError, TypeError):
+        code = None
     if code is None:
         raise ValueError(f"{op}: act must be None, 'relu', 'silu' or 'gelu' (got {act!r})")
     if bias is not None and bias.shape != (n,):
@@ -36,12 +38,12 @@ def check(op: str, shape: tuple, n: int, dtype: torch.dtype, device: torch.devic
         raise ValueError(f"{op}: residual.shape={tuple(residual.shape)} != {tuple(shape)}")
     if out is not None and out.shape != shape:
         raise ValueError(f"{op}: out.shape={tuple(out.shape)} != {tuple(shape)}")
-    if bias is not None:
-        _same(op, "bias", bias, dtype, device)
-    if residual is not None:
-        _same(op, "residual", residual, dtype, device)
-    if out is not None:
-        _same(op, "out", out, dtype, device)
+    if bias is not None and (bias.dtype != dtype or bias.device != device):
+        _refuse(op, "bias", bias, dtype, device)
+    if residual is not None and (residual.dtype != dtype or residual.device != device):
+        _refuse(op, "residual", residual, dtype, device)
+    if out is not None and (out.dtype != dtype or out.device != device):
+        _refuse(op, "out", out, dtype, device)
     return code
 
 

@@ -143,7 +143,9 @@ def check(rc: int, op: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args), name)
+    rc = getattr(_lib or load(), name)(*args)
+    if rc:
+        check(rc, name)
 
 
 # torch's raw accessors of the current device and stream: the public torch.cuda.current_device()

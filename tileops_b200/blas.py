@@ -79,7 +79,8 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
     device = a.device
     code = _epilogue.check(op, (m, n), n, dtype, device, bias, act, residual, out)
     idx = _lib.ensure_device(a, op)
-    _lib.same_device(op, a, b)
+    if b.device != device:
+        _lib.same_device(op, a, b)
     lda = k
     if not a.is_contiguous():
         lda = _row_stride(a)

@@ -18,6 +18,7 @@ import torch
 
 from . import _lib
 
+_ROWS = torch.contiguous_format
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -149,12 +150,11 @@ def act_and_mul_group_quant(a: torch.Tensor, b: torch.Tensor, group_size: int, *
     return q, s
 
 
-def _check_like(op: str, name: str, t: torch.Tensor, dtype: torch.dtype,
-                device: torch.device) -> None:
+def _refuse(op: str, name: str, t: torch.Tensor, dtype: torch.dtype,
+            device: torch.device) -> None:
     if t.dtype != dtype:
         raise TypeError(f"{op}: {name}.dtype={t.dtype} != x.dtype={dtype}")
-    if t.device != device:
-        raise TypeError(f"{op}: all tensors must be on {device} ({name} is on {t.device})")
+    raise TypeError(f"{op}: all tensors must be on {device} ({name} is on {t.device})")
 
 
 def add_rms_norm_group_quant(x: torch.Tensor, weight: torch.Tensor, group_size: int,
@@ -197,31 +197,33 @@ def add_rms_norm_group_quant(x: torch.Tensor, weight: torch.Tensor, group_size: 
     if column_major_scales and x.dim() != 2:
         raise ValueError(f"{op}: column_major_scales needs a 2-D input")
     xd, device = x.dtype, x.device
-    _check_like(op, "weight", weight, xd, device)
+    if weight.dtype != xd or weight.device != device:
+        _refuse(op, "weight", weight, xd, device)
     if residual is not None:
         if residual.shape != x.shape:
             raise ValueError(f"{op}: residual.shape={tuple(residual.shape)} != "
                              f"x.shape={tuple(x.shape)}")
-        _check_like(op, "residual", residual, xd, device)
+        if residual.dtype != xd or residual.device != device:
+            _refuse(op, "residual", residual, xd, device)
     if residual_out is not None:
         if residual is None:
             raise ValueError(f"{op}: residual_out needs a residual")
         if residual_out.shape != x.shape:
             raise ValueError(f"{op}: residual_out.shape={tuple(residual_out.shape)} != "
                              f"x.shape={tuple(x.shape)}")
-        _check_like(op, "residual_out", residual_out, xd, device)
+        if residual_out.dtype != xd or residual_out.device != device:
+            _refuse(op, "residual_out", residual_out, xd, device)
     idx = _lib.ensure_device(x, op)
     if xd not in _DTYPES:
         raise TypeError(f"{op}: unsupported dtype {xd} (float32, float16 and bfloat16 are "
                         "supported)")
-    lead = x.shape[:-1]
     rows = x.numel() // cols if cols else 0
     ldx = ldr = ldh = cols
     if not x.is_contiguous():
         ldx = _row_stride(x)
         if ldx is None:
             x, ldx = x.contiguous(), cols
-    q = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
+    q = torch.empty_like(x, dtype=dtype, memory_format=_ROWS)
     dst = None
     if residual is not None:
         if not residual.is_contiguous():
@@ -231,12 +233,12 @@ def add_rms_norm_group_quant(x: torch.Tensor, weight: torch.Tensor, group_size: 
         if residual_out is not None:
             ldh = cols if residual_out.is_contiguous() else _row_stride(residual_out)
         if residual_out is None or ldh is None:
-            dst, ldh = torch.empty_like(x, memory_format=torch.contiguous_format), cols
+            dst, ldh = torch.empty_like(x, memory_format=_ROWS), cols
         else:
             dst = residual_out
     if not weight.is_contiguous():
         weight = weight.contiguous()
-    s = x.new_empty((*lead, cols // group_size), dtype=torch.float32)
+    s = torch.empty((*x.shape[:-1], cols // group_size), dtype=torch.float32, device=device)
     _lib.call("to_add_rms_norm_group_quant", x.data_ptr(), ldx, _lib.ptr(residual), ldr,
               weight.data_ptr(), _lib.DTYPE_CODES[xd], rows, cols, group_size, eps, quant_eps,
               1 if use_ue8m0 else 0, 1 if column_major_scales else 0, code, q.data_ptr(),
