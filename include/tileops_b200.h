@@ -357,8 +357,8 @@ TO_API int to_act_and_mul_group_quant(const void* a, const void* b, int dtype, i
  * sqrt(mean(h^2) + eps) * weight, scale = max(max|y|, quant_eps) / qmax per group of group_size
  * columns (group_size divides cols; q_dtype TO_E4M3: qmax 448, ue8m0 and column_major as
  * to_per_token_group_quant_fp8; TO_I8: 127), q [rows, cols] the codes of y / scale, dense. fp32
- * throughout; y is not rounded to dtype. h rounded to dtype goes to residual_out unless NULL
- * (x or residual itself allowed). x, residual, residual_out rows ldx, ldr, ldh apart; weight
+ * throughout; y is not rounded to dtype. h rounded to dtype goes to residual_out, given exactly
+ * when residual is (x or residual itself allowed). x, residual, residual_out rows ldx, ldr, ldh apart; weight
  * [cols]; all four of dtype F32, F16 or BF16. */
 TO_API int to_add_rms_norm_group_quant(const void* x, int64_t ldx, const void* residual,
                                        int64_t ldr, const void* weight, int dtype, int64_t rows,

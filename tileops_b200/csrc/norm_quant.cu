@@ -1,14 +1,17 @@
 // Residual add, root-mean-square norm and 8-bit quantisation of a row in one pass:
-//   h = x + r;  rstd = (mean(h^2) + eps)^(-1/2);  y = (h rstd) w
+//   h = x + r;  rstd = (mean(h^2) + eps)^(-1/2);  y = (h w) rstd
 //   per group of G columns: s = max(max|y|, quant_eps) / qmax, q = e4m3 or int8 codes of y / s
 // and h, rounded to the input type, as the next residual. The sums, the norm and the quotients are
 // fp32; nothing is rounded to the input type on the way to the codes.
 //
-// Bound by HBM: 2 + 2 B read, 2 + 1 B written per element (16-bit input), so the row stays in
-// registers between its reduction and its codes and x, r are read once. A team of threads (whole
-// warps) holds a row, MAXV 16-byte packs per thread; the group maxima are shuffles where a group
-// is a power-of-two number of packs within a warp, the team's reduction where it is the row, and
-// shared-memory maxima (order-independent) for any other group size.
+// rstd is one factor of a whole row, so what waits for the row's sum is one number: p = h w stays in
+// registers, max|y| = rstd max|p| per group, and a code is the code of p c with c = rstd / s.
+//
+// Bound by HBM: 2 + 2 B read, 2 + 1 B written per element (16-bit input); x and r are read once. A
+// team of threads (whole warps) holds a row, MAXV 16-byte packs per thread; the group maxima are
+// shuffles where a group is a power-of-two number of packs within a warp, the team's reduction
+// (with the sum's) where it is the row, and shared-memory maxima (order-independent) for any other
+// group size. Few rows take one or two packs per thread: their time is the latency of one load.
 #include <algorithm>
 
 #include "quant_codes.cuh"
@@ -22,234 +25,311 @@ struct NormArgs {
   const void* x;
   const void* r;       // null: no residual
   const void* w;
-  void* h;             // null: no residual output; may be x or r
+  void* h;             // residual output, null without r; may be x or r
   uint8_t* q;
   float* scales;
   int64_t rows, cols, ldx, ldr, ldh;
   int G;               // columns per group
   int team;            // threads per row, a multiple of 32
+  int rows_per_block, nvec, groups, lanes_log2;
   float eps, quant_eps, qmax;
+  float floor_factor;  // qmax / quant_eps
   int ue8m0;
   ScaleLayout sl;
 };
 
-// Maximum key / sum over the team. `red`: one word per warp of the CTA. Every thread of the CTA
-// calls it; the barrier in front separates uses of `red`.
-template <typename R, typename F>
-__device__ __forceinline__ R team_reduce(R v, int team, R* red, F op) {
-  const int warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if (team == 32) return v;
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[warp] = v;
-  __syncthreads();
-  const int warps = team >> 5, w0 = warp / warps * warps;
-  R t = red[w0];
-  for (int i = 1; i < warps; ++i) t = op(t, red[w0 + i]);
-  return t;
+// max(|v|, m), NaN when either is.
+__device__ __forceinline__ float max_abs_nan(float v, float m) {
+  asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %1;\n\tmax.NaN.f32 %0, t, %2;\n\t}" : "=f"(m) : "f"(v), "f"(m));
+  return m;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(a), "f"(b));
+  return a;
 }
 
-template <typename T, int Q, int V, int MAXV, int MODE>
-__global__ void __launch_bounds__(1024) k_norm_quant(const NormArgs a) {
-  __shared__ float red_sum[32];
-  __shared__ unsigned red_max[32];
+// scale = clamp(max|y|, min = quant_eps) / qmax; a NaN maximum passes through unchanged.
+template <int Q>
+__device__ __forceinline__ float scale_of(float maxp, float rstd, const NormArgs& a) {
+  const float m = maxp * rstd;
+  if (isnan(m)) return __uint_as_float(0x7FC00000u);
+  float s = __fdiv_rn(fmaxf(m, a.quant_eps), a.qmax);
+  if (Q == kQE4M3 && a.ue8m0) s = ue8m0_round(s);
+  return s;
+}
+
+// The factor c of a group, rstd / s up to a few roundings: qmax / max|p|, or what the floor of the
+// scale leaves. 0 stands for the groups whose codes need a division each (a NaN or an infinity, or
+// numbers near the ends of fp32's range). Every lane works one out per pack, so it is short.
+template <int Q>
+__device__ __forceinline__ float code_factor(float maxp, float rstd, const NormArgs& a) {
+  const float m = maxp * rstd;
+  float c = m > a.quant_eps ? __fdividef(a.qmax, maxp) : rstd * a.floor_factor;
+  if (Q == kQE4M3 && a.ue8m0) c = __fdividef(rstd, scale_of<Q>(maxp, rstd, a));
+  const bool plain = m <= 1e30f && maxp <= 1e30f && (maxp >= 1e-30f || maxp == 0.f) &&
+                     c <= 1e30f;  // false for NaN
+  return plain ? c : 0.f;
+}
+
+// The codes of V values p c. With a factor every value is finite and |p c| <= qmax (1 + 2^-21),
+// which saturates (e4m3) or rounds (int8) to qmax.
+template <int Q, int V>
+__device__ __forceinline__ Pack<uint8_t, V> codes_of(const Pack<float, V>& f, float c) {
+  Pack<uint8_t, V> o;
+  if constexpr (V == 1) {
+    const float z = f.v[0] * c;
+    o.v[0] = Q == kQE4M3 ? f32_to_e4m3(z) : (uint8_t)__float_as_uint(z + 12582912.0f);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V / 4; ++k) {
+      const float* z = f.v + 4 * k;
+      uint32_t lo, hi;
+      if constexpr (Q == kQE4M3) {
+        lo = f32x2_to_e4m3x2(z[0] * c, z[1] * c);
+        hi = f32x2_to_e4m3x2(z[2] * c, z[3] * c);
+      } else {  // the low byte of z + 1.5 x 2^23 is rint(z)
+        lo = __byte_perm(__float_as_uint(fmaf(z[0], c, 12582912.0f)),
+                         __float_as_uint(fmaf(z[1], c, 12582912.0f)), 0x0040);
+        hi = __byte_perm(__float_as_uint(fmaf(z[2], c, 12582912.0f)),
+                         __float_as_uint(fmaf(z[3], c, 12582912.0f)), 0x0040);
+      }
+      reinterpret_cast<uint32_t*>(o.v)[k] = __byte_perm(lo, hi, 0x5410);
+    }
+  }
+  return o;
+}
+// One code by division, for the groups without a factor. Out of line: it is never fetched else.
+template <int Q>
+__device__ __noinline__ uint8_t divided_code(float p, float rstd, float s) {
+  const float z = __fdiv_rn(p * rstd, s);
+  if (Q == kQE4M3) return isnan(z) ? (uint8_t)0x7F : f32_to_e4m3(fminf(fmaxf(z, -448.f), 448.f));
+  return (uint8_t)rne_clamp_i8(z);
+}
+
+// Threads of a block at most: four packs a thread want 80 registers, fewer packs fit 64.
+template <int V, int MAXV> constexpr int kBlockMax = V > 1 && MAXV == 4 ? 384 : 1024;
+
+// RES: with a residual and its output. Loads are not guarded but clamped (rows and packs past the
+// end re-read the last and count as zero), so that all of a thread's loads go out together.
+template <typename T, int Q, int V, int MAXV, int MODE, bool RES>
+__global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlockMax<V, MAXV> == 384 ? 2 : 1)
+    k_norm_quant(const __grid_constant__ NormArgs a) {
+  __shared__ float red[2][32];
   extern __shared__ unsigned gmax[];  // kGroupShared: [rows of the CTA][groups]
   // Launched as a programmatic dependent: blocks may start while the previous kernel drains, and
   // wait for its completion before they touch memory.
   grid_dependents_launch();
   grid_dependency_wait();
   const int team = a.team;
-  const int tid = (int)threadIdx.x % team, local = (int)threadIdx.x / team;
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / team) + local;
+  int tid = (int)threadIdx.x, local = 0;
+  if (team < (int)blockDim.x) {
+    local = tid / team;
+    tid -= local * team;
+  }
+  const int64_t row = (int64_t)blockIdx.x * a.rows_per_block + local;
   const bool active = row < a.rows;
-  const int nvec = (int)(a.cols / V);
-  const int groups = (int)(a.cols / a.G);
-  const T* x = (const T*)a.x + row * a.ldx;
-  const T* r = a.r ? (const T*)a.r + row * a.ldr : nullptr;
+  const int nvec = a.nvec, groups = a.groups;
+  const int64_t lrow = active ? row : a.rows - 1;
+  const T* x = (const T*)a.x + lrow * a.ldx;
+  const T* r = RES ? (const T*)a.r + lrow * a.ldr : nullptr;
   const T* w = (const T*)a.w;
-  T* h = a.h ? (T*)a.h + row * a.ldh : nullptr;
+  T* h = RES ? (T*)a.h + lrow * a.ldh : nullptr;
+  uint8_t* q = a.q + lrow * a.cols;
   using F = Pack<float, V>;
 
-  auto load_h = [&](int v) {
+  auto add = [&](const Pack<T, V>& px, const Pack<T, V>& pr) {
     F o;
-    const Pack<T, V> px = ld_pack<T, V>(x + (int64_t)v * V);
-    if (r != nullptr) {
-      const Pack<T, V> pr = ld_pack<T, V>(r + (int64_t)v * V);
 #pragma unroll
-      for (int j = 0; j < V; ++j) o.v[j] = to_f32(px.v[j]) + to_f32(pr.v[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) o.v[j] = to_f32(px.v[j]);
+    for (int j = 0; j < V; ++j) {
+      o.v[j] = to_f32(px.v[j]);
+      if constexpr (RES) o.v[j] += to_f32(pr.v[j]);
     }
     return o;
   };
   auto store_h = [&](int v, const F& f) {
-    if (h == nullptr) return;
-    Pack<T, V> o;
+    if constexpr (RES) {
+      Pack<T, V> o;
 #pragma unroll
-    for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(f.v[j]);
-    st_pack<T, V>(h + (int64_t)v * V, o);
-  };
-
-  // h of this thread's packs, and the row's sum of squares. Packs past MAXV are re-read in each
-  // pass; their h is stored in the last one, since it may overwrite x or r.
-  F y[MAXV];
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < MAXV; ++i) {
-    const int v = tid + i * team;
-    if (active && v < nvec) y[i] = load_h(v);
-  }
-#pragma unroll
-  for (int i = 0; i < MAXV; ++i) {
-    const int v = tid + i * team;
-    if (active && v < nvec) {
-      store_h(v, y[i]);
-#pragma unroll
-      for (int j = 0; j < V; ++j) ss = fmaf(y[i].v[j], y[i].v[j], ss);
+      for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(f.v[j]);
+      st_pack<T, V>(h + (int64_t)v * V, o);
     }
-  }
-  for (int v = tid + MAXV * team; active && v < nvec; v += team) {
-    const F f = load_h(v);
+  };
+  auto load_h = [&](int v) {
+    Pack<T, V> pr;
+    if constexpr (RES) pr = ld_pack<T, V>(r + (int64_t)v * V);
+    return add(ld_pack<T, V>(x + (int64_t)v * V), pr);
+  };
+  auto weigh = [&](F& f, const Pack<T, V>& pw) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f.v[j] *= to_f32(pw.v[j]);
+  };
+  float ss = 0.f, rowmax = 0.f;
+  auto square = [&](const F& f) {
 #pragma unroll
     for (int j = 0; j < V; ++j) ss = fmaf(f.v[j], f.v[j], ss);
+  };
+  auto max_of = [&](const F& f, float m) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) m = max_abs_nan(f.v[j], m);
+    return m;
+  };
+
+  // Packs past MAXV are re-read in each pass; their h is stored in the last one, since it may
+  // overwrite x or r.
+  F y[MAXV];
+  {
+    Pack<T, V> px[MAXV], pr[MAXV];
+#pragma unroll
+    for (int i = 0; i < MAXV; ++i) {
+      const int v = min(tid + i * team, nvec - 1);
+      px[i] = ld_pack<T, V>(x + (int64_t)v * V);
+      if constexpr (RES) pr[i] = ld_pack<T, V>(r + (int64_t)v * V);
+    }
+#pragma unroll
+    for (int i = 0; i < MAXV; ++i) {
+      const int v = tid + i * team;
+      const Pack<T, V> pw = ld_pack<T, V>(w + (int64_t)min(v, nvec - 1) * V);
+      y[i] = add(px[i], pr[i]);
+      if (v < nvec) {
+        if (active) store_h(v, y[i]);
+        square(y[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[i].v[j] = 0.f;
+      }
+      weigh(y[i], pw);
+      if constexpr (MODE == kGroupRow)
+        if (v < nvec) rowmax = max_of(y[i], rowmax);
+    }
   }
-  ss = team_reduce(ss, team, red_sum, [](float p, float q) { return p + q; });
+  for (int v = tid + MAXV * team; v < nvec; v += team) {
+    F f = load_h(v);
+    square(f);
+    if constexpr (MODE == kGroupRow) {
+      weigh(f, ld_pack<T, V>(w + (int64_t)v * V));
+      rowmax = max_of(f, rowmax);
+    }
+  }
+  // The team's sum, and with one scale per row its maximum.
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if constexpr (MODE == kGroupRow) rowmax = max_nan(rowmax, __shfl_xor_sync(0xffffffffu, rowmax, o));
+  }
+  if (team > 32) {
+    const int warp = threadIdx.x >> 5, warps = team >> 5, w0 = local * warps;
+    if ((threadIdx.x & 31) == 0) {
+      red[0][warp] = ss;
+      if constexpr (MODE == kGroupRow) red[1][warp] = rowmax;
+    }
+    __syncthreads();
+    // Lane l takes warp l's number; every warp adds them up alike.
+    const int l = threadIdx.x & 31;
+    ss = l < warps ? red[0][w0 + l] : 0.f;
+    if constexpr (MODE == kGroupRow) rowmax = l < warps ? red[1][w0 + l] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if constexpr (MODE == kGroupRow)
+        rowmax = max_nan(rowmax, __shfl_xor_sync(0xffffffffu, rowmax, o));
+    }
+  }
   const float rstd = __frsqrt_rn(ss / (float)a.cols + a.eps);
 
-  auto norm = [&](int v, F f) {
-    const Pack<T, V> pw = ld_pack<T, V>(w + (int64_t)v * V);
-#pragma unroll
-    for (int j = 0; j < V; ++j) f.v[j] = f.v[j] * rstd * to_f32(pw.v[j]);
-    return f;
-  };
-  auto key_of = [&](const F& f) {
-    unsigned k = 0u;
-#pragma unroll
-    for (int j = 0; j < V; ++j) k = max(k, abs_key(f.v[j]));
-    return k;
-  };
-  // scale = clamp(absmax, min = quant_eps) / qmax; a NaN absmax passes through unchanged.
-  auto scale_of = [&](unsigned key) {
-    const float m = __uint_as_float(key);
-    if (isnan(m)) return m;
-    float s = __fdiv_rn(fmaxf(m, a.quant_eps), a.qmax);
-    if (Q == kQE4M3 && a.ue8m0) s = ue8m0_round(s);
-    return s;
-  };
   auto put_scale = [&](int g, float s) { a.scales[scale_offset(row * groups + g, a.sl)] = s; };
-  auto emit = [&](int v, const F& f, float s) {
+  // Codes of a pack whose group has the maximum maxp.
+  auto emit = [&](int v, const F& f, float maxp, float c) {
     Pack<uint8_t, V> o;
-    if (s >= 1.2e-38f && s <= 8.0e37f) {
-      bracket_codes<Q>(f, make_bracket(s), s, o);
+    if (c != 0.f) {
+      o = codes_of<Q, V>(f, c);
     } else {
+      const float s = scale_of<Q>(maxp, rstd, a);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float z = __fdiv_rn(f.v[j], s);
-        if (Q == kQE4M3)
-          o.v[j] = isnan(z) ? (uint8_t)0x7F : f32_to_e4m3(fminf(fmaxf(z, -448.f), 448.f));
-        else
-          o.v[j] = (uint8_t)rne_clamp_i8(z);
-      }
+      for (int j = 0; j < V; ++j) o.v[j] = divided_code<Q>(f.v[j], rstd, s);
     }
-    st_pack<uint8_t, V>(a.q + row * a.cols + (int64_t)v * V, o);
+    st_pack<uint8_t, V>(q + (int64_t)v * V, o);
   };
-
-#pragma unroll
-  for (int i = 0; i < MAXV; ++i) {
-    const int v = tid + i * team;
-    if (active && v < nvec) y[i] = norm(v, y[i]);
-  }
 
   if constexpr (MODE == kGroupLanes) {
     // A group is `lanes` consecutive packs: packs of one i are consecutive over the team's
     // threads and the team is whole warps, so a group never leaves its warp.
-    const int lanes = a.G / V;
-    const int shift = 31 - __clz(lanes);
+    const int shift = a.lanes_log2;
+    auto group_max = [&](float m) {
+      for (int o = 1 << shift >> 1; o > 0; o >>= 1)
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+      return m;
+    };
+    auto finish = [&](int v, const F& f, float m) {
+      if (!active || v >= nvec) return;
+      if ((v & ((1 << shift) - 1)) == 0) put_scale(v >> shift, scale_of<Q>(m, rstd, a));
+      emit(v, f, m, code_factor<Q>(m, rstd, a));
+    };
 #pragma unroll
-    for (int i = 0; i < MAXV; ++i) {
-      const int v = tid + i * team;
-      const bool have = active && v < nvec;
-      const unsigned k = warp_max_key(have ? key_of(y[i]) : 0u, lanes);
-      if (have) {
-        const float s = scale_of(k);
-        if ((v & (lanes - 1)) == 0) put_scale(v >> shift, s);
-        emit(v, y[i], s);
-      }
-    }
-    const int rounds = (nvec + team - 1) / team;  // uniform trip count: the shuffles need all lanes
-    for (int i = MAXV; i < rounds; ++i) {
-      const int v = tid + i * team;
-      const bool have = active && v < nvec;
+    for (int i = 0; i < MAXV; ++i)
+      finish(tid + i * team, y[i], group_max(max_of(y[i], 0.f)));
+    // uniform trip count: the shuffles need all lanes
+    for (int v = tid + MAXV * team; v - tid < nvec; v += team) {
       F f;
-      if (have) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) f.v[j] = 0.f;
+      if (v < nvec) {
         f = load_h(v);
-        store_h(v, f);
-        f = norm(v, f);
+        if (active) store_h(v, f);
+        weigh(f, ld_pack<T, V>(w + (int64_t)v * V));
       }
-      const unsigned k = warp_max_key(have ? key_of(f) : 0u, lanes);
-      if (have) {
-        const float s = scale_of(k);
-        if ((v & (lanes - 1)) == 0) put_scale(v >> shift, s);
-        emit(v, f, s);
-      }
+      finish(v, f, group_max(max_of(f, 0.f)));
     }
   } else {
     unsigned* gm = gmax + local * groups;
-    if constexpr (MODE == kGroupShared) {
+    if constexpr (MODE == kGroupRow) {
+      if (active && tid == 0) put_scale(0, scale_of<Q>(rowmax, rstd, a));
+    } else {
       for (int g = tid; g < groups; g += team) gm[g] = 0u;
       __syncthreads();
-    }
-    unsigned k = 0u;
-    auto note = [&](int v, const F& f) {
-      if constexpr (MODE == kGroupRow) k = max(k, key_of(f));
-      else atomicMax(gm + (int)(((int64_t)v * V) / a.G), key_of(f));  // V divides G
-    };
+      // Bit patterns of non-negative floats order as the floats, NaN above all.
+      auto note = [&](int v, const F& f) {
+        atomicMax(gm + (v * V) / a.G, __float_as_uint(max_of(f, 0.f)));
+      };
 #pragma unroll
-    for (int i = 0; i < MAXV; ++i) {
-      const int v = tid + i * team;
-      if (active && v < nvec) note(v, y[i]);
-    }
-    for (int v = tid + MAXV * team; active && v < nvec; v += team) note(v, norm(v, load_h(v)));
-    float s = 0.f;
-    if constexpr (MODE == kGroupRow) {
-      k = team_reduce(k, team, red_max, [](unsigned p, unsigned q) { return max(p, q); });
-      s = scale_of(k);
-      if (active && tid == 0) put_scale(0, s);
-    } else {
-      __syncthreads();
-      for (int g = tid; active && g < groups; g += team) {
-        const float t = scale_of(gm[g]);
-        put_scale(g, t);
-        gm[g] = __float_as_uint(t);
+      for (int i = 0; i < MAXV; ++i)
+        if (tid + i * team < nvec) note(tid + i * team, y[i]);
+      for (int v = tid + MAXV * team; v < nvec; v += team) {
+        F f = load_h(v);
+        weigh(f, ld_pack<T, V>(w + (int64_t)v * V));
+        note(v, f);
       }
       __syncthreads();
+      for (int g = tid; active && g < groups; g += team)
+        put_scale(g, scale_of<Q>(__uint_as_float(gm[g]), rstd, a));
     }
-    auto scale_at = [&](int v) {
-      if constexpr (MODE == kGroupRow) return s;
-      else return __uint_as_float(gm[(int)(((int64_t)v * V) / a.G)]);
+    const float c_row = MODE == kGroupRow ? code_factor<Q>(rowmax, rstd, a) : 0.f;
+    auto finish = [&](int v, const F& f) {
+      if constexpr (MODE == kGroupRow) {
+        emit(v, f, rowmax, c_row);
+      } else {
+        const float m = __uint_as_float(gm[(v * V) / a.G]);
+        emit(v, f, m, code_factor<Q>(m, rstd, a));
+      }
     };
 #pragma unroll
-    for (int i = 0; i < MAXV; ++i) {
-      const int v = tid + i * team;
-      if (active && v < nvec) emit(v, y[i], scale_at(v));
-    }
+    for (int i = 0; i < MAXV; ++i)
+      if (active && tid + i * team < nvec) finish(tid + i * team, y[i]);
     for (int v = tid + MAXV * team; active && v < nvec; v += team) {
-      const F f = load_h(v);
-      const float sv = scale_at(v);
-      const F z = norm(v, f);
+      F f = load_h(v);
       store_h(v, f);
-      emit(v, z, sv);
+      weigh(f, ld_pack<T, V>(w + (int64_t)v * V));
+      finish(v, f);
     }
   }
 }
 
 template <typename T, int Q, int V, int MAXV, int MODE>
 int launch_norm(NormArgs a, cudaStream_t st) {
+  auto kern = a.h != nullptr ? k_norm_quant<T, Q, V, MAXV, MODE, true>
+                             : k_norm_quant<T, Q, V, MAXV, MODE, false>;
   const int64_t nvec = a.cols / V;
   int64_t team = ceil_div(ceil_div(nvec, MAXV), 32) * 32;
-  if (team > 1024) team = 1024;
+  if (team > kBlockMax<V, MAXV>) team = kBlockMax<V, MAXV>;
   a.team = (int)team;
   // Small rows share a CTA of up to 256 threads.
   int64_t per_cta = std::max<int64_t>(1, 256 / team);
@@ -261,10 +341,14 @@ int launch_norm(NormArgs a, cudaStream_t st) {
     if (smem > 200 * 1024)
       return fail(TO_EUNSUPPORTED, "add_rms_norm_group_quant: %lld groups in a row (at most 51200)",
                   (long long)groups);
-    const cudaError_t e =
-        ensure_smem_attr((const void*)k_norm_quant<T, Q, V, MAXV, MODE>, 200 * 1024);
+    const cudaError_t e = ensure_smem_attr((const void*)kern, 200 * 1024);
     if (e != cudaSuccess) return cuda_fail(e, "add_rms_norm_group_quant: shared memory attribute");
   }
+  a.rows_per_block = (int)per_cta;
+  a.nvec = (int)nvec;
+  a.groups = (int)groups;
+  a.lanes_log2 = 0;
+  while (MODE == kGroupLanes && (V << a.lanes_log2) < a.G) ++a.lanes_log2;
   const int64_t blocks = ceil_div(a.rows, per_cta);
   if (blocks > INT32_MAX) return fail(TO_EUNSUPPORTED, "add_rms_norm_group_quant: too many rows");
   cudaLaunchConfig_t cfg = {};
@@ -277,7 +361,7 @@ int launch_norm(NormArgs a, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_norm_quant<T, Q, V, MAXV, MODE>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return cuda_fail(e, "add_rms_norm_group_quant launch");
   return check_launch("add_rms_norm_group_quant");
 }
@@ -294,11 +378,22 @@ int launch_norm_any(const NormArgs& a, cudaStream_t st) {
     return launch_norm<T, Q, 1, 8, kGroupShared>(a, st);
   }
   const int lanes = a.G / VV;
-  if (a.G == a.cols && lanes > 32) return launch_norm<T, Q, VV, 4, kGroupRow>(a, st);
-  if (lanes <= 32 && (lanes & (lanes - 1)) == 0)
-    return launch_norm<T, Q, VV, 4, kGroupLanes>(a, st);
-  if (a.G == a.cols) return launch_norm<T, Q, VV, 4, kGroupRow>(a, st);
-  return launch_norm<T, Q, VV, 4, kGroupShared>(a, st);
+  const int mode = lanes <= 32 && (lanes & (lanes - 1)) == 0 ? kGroupLanes
+                   : a.G == a.cols                          ? kGroupRow
+                                                            : kGroupShared;
+  if (mode == kGroupShared) return launch_norm<T, Q, VV, 4, kGroupShared>(a, st);
+  // Packs per thread: few rows (two per SM) take as few as keep a row in one block, for latency;
+  // many take four, for bytes in flight at few threads, or two where the row needs 1024 threads.
+  const int64_t nvec = a.cols / VV;
+  const int maxv = a.rows <= 2 * sm_count() ? (nvec <= 1024 ? 1 : 2) : (nvec <= 4 * 384 ? 4 : 2);
+  auto run = [&](auto m) {
+    constexpr int MODE = decltype(m)::value;
+    if (maxv == 1) return launch_norm<T, Q, VV, 1, MODE>(a, st);
+    if (maxv == 2) return launch_norm<T, Q, VV, 2, MODE>(a, st);
+    return launch_norm<T, Q, VV, 4, MODE>(a, st);
+  };
+  return mode == kGroupLanes ? run(std::integral_constant<int, kGroupLanes>{})
+                             : run(std::integral_constant<int, kGroupRow>{});
 }
 
 }  // namespace
@@ -322,6 +417,8 @@ extern "C" int to_add_rms_norm_group_quant(
     return fail(TO_EINVAL, "%s: ue8m0 / column-major scales are FP8 options", op);
   if (rows == 0 || cols == 0) return TO_OK;
   if (!x || !weight || !q || !scales) return fail(TO_EINVAL, "%s: null pointer", op);
+  if ((residual == nullptr) != (residual_out == nullptr))
+    return fail(TO_EINVAL, "%s: a residual and its output go together", op);
   NormArgs a;
   a.x = x;
   a.r = residual;
@@ -339,6 +436,7 @@ extern "C" int to_add_rms_norm_group_quant(
   a.eps = eps;
   a.quant_eps = quant_eps;
   a.qmax = q_dtype == TO_E4M3 ? 448.0f : 127.0f;
+  a.floor_factor = a.qmax / quant_eps;
   a.ue8m0 = ue8m0;
   a.sl = ScaleLayout{column_major ? rows : 0, column_major ? cols / group_size : 1};
   cudaStream_t st = (cudaStream_t)stream;
