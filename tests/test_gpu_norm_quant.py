@@ -71,6 +71,37 @@ def test_definition(cuda, codes, dt, rows, cols, g):
     check(x, w, r, g, codes, got)
 
 
+@pytest.mark.parametrize("codes", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,cols,g", [
+    # rows past a few per SM run on persistent blocks: a last block part full, one and several rows
+    # per block, columns that leave threads idle, rows of one and of two blocks' shared memory
+    (593, 256, 256), (1201, 384, 128), (777, 1024, 64), (650, 5120, 5120), (700, 11008, 128),
+    (601, 16384, 16384), (600, 8192, 8192), (2000, 32, 32), (3000, 64, 16),
+])
+def test_many_rows(cuda, codes, dt, rows, cols, g):
+    gen = torch.Generator(device=cuda).manual_seed(rows + cols)
+    x = torch.randn(rows, cols, generator=gen, device=cuda).to(dt)
+    r = (torch.randn(rows, cols, generator=gen, device=cuda) * 3).to(dt)
+    w = (1 + 0.3 * torch.randn(cols, generator=gen, device=cuda)).to(dt)
+    x[7] = 0
+    x[11, 3] = float("inf")
+    keep = [i for i in range(rows) if i != 11]
+    q, s = tob.add_rms_norm_group_quant(x, w, g, dtype=codes)
+    check(x[keep], w, None, g, codes, (q[keep], s[keep]))
+    assert bool(torch.isnan(s[11, 3 // g]))
+    r[11] = -x[11].clamp(max=1)
+    x[11, 3] = 1
+    want = tob.add_rms_norm_group_quant(x, w, g, r, dtype=codes)
+    check(x, w, r, g, codes, want)
+    wide = torch.full((rows, cols + 8), 7, dtype=dt, device=cuda)
+    wide[:, 8:] = r
+    got = tob.add_rms_norm_group_quant(x, w, g, wide[:, 8:], dtype=codes, residual_out=wide[:, 8:])
+    assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8))
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    assert bool((wide[:, :8] == 7).all())
+
+
 @pytest.mark.parametrize("cols,g", [(512, 128), (512, 512), (480, 96), (333, 111), (40960, 128),
                                     (40960, 40960), (40960, 5120)])
 @pytest.mark.parametrize("into", ["x", "residual"])

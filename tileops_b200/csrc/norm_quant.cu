@@ -32,7 +32,7 @@ struct NormArgs {
   int G;               // columns per group
   int team;            // threads per row, a multiple of 32
   int rows_per_block, nvec, groups, lanes_log2;
-  float eps, quant_eps, qmax;
+  float eps, quant_eps, qmax, qmax_inv, cols_inv;
   float floor_factor;  // qmax / quant_eps
   int ue8m0;
   ScaleLayout sl;
@@ -48,12 +48,50 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return a;
 }
 
+// x + r of a pack in fp32. 16-bit values go straight into mixed-precision products with one, which
+// convert and add in the same instruction.
+template <typename T, int V, bool RES>
+__device__ __forceinline__ Pack<float, V> sum_packs(const Pack<T, V>& px, const Pack<T, V>& pr) {
+  Pack<float, V> o;
+  if constexpr (RES && V > 1 && std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2)
+      asm("{\n\t.reg .b16 xl, xh, rl, rh, one;\n\tmov.b32 {xl, xh}, %2;\n\tmov.b32 {rl, rh}, %3;\n\t"
+          "mov.b16 one, 0x3F80;\n\t"
+          "fma.rn.f32.bf16 %0, rl, one, 0f00000000;\n\tfma.rn.f32.bf16 %1, rh, one, 0f00000000;\n\t"
+          "fma.rn.f32.bf16 %0, xl, one, %0;\n\tfma.rn.f32.bf16 %1, xh, one, %1;\n\t}"
+          : "=&f"(o.v[j]), "=&f"(o.v[j + 1])
+          : "r"(*reinterpret_cast<const uint32_t*>(px.v + j)),
+            "r"(*reinterpret_cast<const uint32_t*>(pr.v + j)));
+  } else if constexpr (RES && V > 1 && std::is_same<T, __half>::value) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2)
+      asm("{\n\t.reg .b16 xl, xh, rl, rh, one;\n\tmov.b32 {xl, xh}, %2;\n\tmov.b32 {rl, rh}, %3;\n\t"
+          "mov.b16 one, 0x3C00;\n\t"
+          "fma.rn.f32.f16 %0, rl, one, 0f00000000;\n\tfma.rn.f32.f16 %1, rh, one, 0f00000000;\n\t"
+          "fma.rn.f32.f16 %0, xl, one, %0;\n\tfma.rn.f32.f16 %1, xh, one, %1;\n\t}"
+          : "=&f"(o.v[j]), "=&f"(o.v[j + 1])
+          : "r"(*reinterpret_cast<const uint32_t*>(px.v + j)),
+            "r"(*reinterpret_cast<const uint32_t*>(pr.v + j)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      o.v[j] = to_f32(px.v[j]);
+      if constexpr (RES) o.v[j] += to_f32(pr.v[j]);
+    }
+  }
+  return o;
+}
+
 // scale = clamp(max|y|, min = quant_eps) / qmax; a NaN maximum passes through unchanged.
 template <int Q>
 __device__ __forceinline__ float scale_of(float maxp, float rstd, const NormArgs& a) {
   const float m = maxp * rstd;
   if (isnan(m)) return __uint_as_float(0x7FC00000u);
-  float s = __fdiv_rn(fmaxf(m, a.quant_eps), a.qmax);
+  // The IEEE quotient by the constant: qmax_inv is the rounded reciprocal, one correction makes the
+  // rounded quotient of it (fp32 subnormal results excepted, where it may be one step off).
+  const float n = fmaxf(m, a.quant_eps), t = n * a.qmax_inv;
+  float s = isinf(n) ? n : fmaf(fmaf(-t, a.qmax, n), a.qmax_inv, t);
   if (Q == kQE4M3 && a.ue8m0) s = ue8m0_round(s);
   return s;
 }
@@ -109,8 +147,10 @@ __device__ __noinline__ uint8_t divided_code(float p, float rstd, float s) {
 // Threads of a block at most: four packs a thread want 80 registers, fewer packs fit 64.
 template <int V, int MAXV> constexpr int kBlockMax = V > 1 && MAXV == 4 ? 384 : 1024;
 
-// RES: with a residual and its output. Loads are not guarded but clamped (rows and packs past the
-// end re-read the last and count as zero), so that all of a thread's loads go out together.
+// One block per rows_per_block rows, a team of threads each. RES: with a residual and its output.
+// Loads are not guarded but clamped (rows and packs past the end re-read the last and count as
+// zero), so that all of a thread's loads go out together. 8192 x 8192 bf16 -> e4m3 with residual:
+// 87 us, 5.4 TB/s; a persistent form fed by bulk copies into shared memory ran no faster.
 template <typename T, int Q, int V, int MAXV, int MODE, bool RES>
 __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlockMax<V, MAXV> == 384 ? 2 : 1)
     k_norm_quant(const __grid_constant__ NormArgs a) {
@@ -137,27 +177,28 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlockMax<V, MAXV> == 384 
   uint8_t* q = a.q + lrow * a.cols;
   using F = Pack<float, V>;
 
-  auto add = [&](const Pack<T, V>& px, const Pack<T, V>& pr) {
-    F o;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      o.v[j] = to_f32(px.v[j]);
-      if constexpr (RES) o.v[j] += to_f32(pr.v[j]);
-    }
-    return o;
-  };
   auto store_h = [&](int v, const F& f) {
     if constexpr (RES) {
       Pack<T, V> o;
+      if constexpr (V > 1 && std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(f.v[j]);
+        for (int j = 0; j < V; j += 2)
+          *reinterpret_cast<__nv_bfloat162*>(o.v + j) = __floats2bfloat162_rn(f.v[j], f.v[j + 1]);
+      } else if constexpr (V > 1 && std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int j = 0; j < V; j += 2)
+          *reinterpret_cast<__half2*>(o.v + j) = __floats2half2_rn(f.v[j], f.v[j + 1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(f.v[j]);
+      }
       st_pack<T, V>(h + (int64_t)v * V, o);
     }
   };
   auto load_h = [&](int v) {
     Pack<T, V> pr;
     if constexpr (RES) pr = ld_pack<T, V>(r + (int64_t)v * V);
-    return add(ld_pack<T, V>(x + (int64_t)v * V), pr);
+    return sum_packs<T, V, RES>(ld_pack<T, V>(x + (int64_t)v * V), pr);
   };
   auto weigh = [&](F& f, const Pack<T, V>& pw) {
 #pragma unroll
@@ -189,17 +230,16 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlockMax<V, MAXV> == 384 
     for (int i = 0; i < MAXV; ++i) {
       const int v = tid + i * team;
       const Pack<T, V> pw = ld_pack<T, V>(w + (int64_t)min(v, nvec - 1) * V);
-      y[i] = add(px[i], pr[i]);
+      y[i] = sum_packs<T, V, RES>(px[i], pr[i]);
       if (v < nvec) {
         if (active) store_h(v, y[i]);
         square(y[i]);
-      } else {
+        weigh(y[i], pw);
+        if constexpr (MODE == kGroupRow) rowmax = max_of(y[i], rowmax);
+      } else if constexpr (MODE == kGroupLanes) {  // counts as zero in the shuffled maxima
 #pragma unroll
         for (int j = 0; j < V; ++j) y[i].v[j] = 0.f;
       }
-      weigh(y[i], pw);
-      if constexpr (MODE == kGroupRow)
-        if (v < nvec) rowmax = max_of(y[i], rowmax);
     }
   }
   for (int v = tid + MAXV * team; v < nvec; v += team) {
@@ -234,9 +274,13 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlockMax<V, MAXV> == 384 
         rowmax = max_nan(rowmax, __shfl_xor_sync(0xffffffffu, rowmax, o));
     }
   }
-  const float rstd = __frsqrt_rn(ss / (float)a.cols + a.eps);
+  const float rstd = rsqrtf(fmaf(ss, a.cols_inv, a.eps));
 
-  auto put_scale = [&](int g, float s) { a.scales[scale_offset(row * groups + g, a.sl)] = s; };
+  float* scales = a.scales + lrow * groups;
+  auto put_scale = [&](int g, float s) {
+    if (a.sl.cm_rows > 0) a.scales[scale_offset(row * groups + g, a.sl)] = s;
+    else scales[g] = s;
+  };
   // Codes of a pack whose group has the maximum maxp.
   auto emit = [&](int v, const F& f, float maxp, float c) {
     Pack<uint8_t, V> o;
@@ -255,8 +299,9 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlockMax<V, MAXV> == 384 
     // threads and the team is whole warps, so a group never leaves its warp.
     const int shift = a.lanes_log2;
     auto group_max = [&](float m) {
-      for (int o = 1 << shift >> 1; o > 0; o >>= 1)
-        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+      for (int b = 0; b < 5; ++b)
+        if (b < shift) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1 << b));
       return m;
     };
     auto finish = [&](int v, const F& f, float m) {
@@ -264,9 +309,31 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlockMax<V, MAXV> == 384 
       if ((v & ((1 << shift) - 1)) == 0) put_scale(v >> shift, scale_of<Q>(m, rstd, a));
       emit(v, f, m, code_factor<Q>(m, rstd, a));
     };
+    if (MAXV > 1 && shift >= 2) {
+      // Lane i of a group works out the scale and the factor of the thread's i-th pack, once per
+      // row instead of once per pack.
+      static_assert(MAXV <= 4 || V == 1, "lane i of a group of four or more");
+      float m[MAXV];
 #pragma unroll
-    for (int i = 0; i < MAXV; ++i)
-      finish(tid + i * team, y[i], group_max(max_of(y[i], 0.f)));
+      for (int i = 0; i < MAXV; ++i) m[i] = group_max(max_of(y[i], 0.f));
+      const int lane = threadIdx.x & 31, i_mine = lane & ((1 << shift) - 1);
+      float mine = m[0];
+#pragma unroll
+      for (int i = 1; i < MAXV; ++i) mine = i == i_mine ? m[i] : mine;
+      const int v_mine = tid + i_mine * team;
+      if (active && i_mine < MAXV && v_mine < nvec)
+        put_scale(v_mine >> shift, scale_of<Q>(mine, rstd, a));
+      const float c = code_factor<Q>(mine, rstd, a);
+#pragma unroll
+      for (int i = 0; i < MAXV; ++i) {
+        const float ci = __shfl_sync(0xffffffffu, c, lane - i_mine + i);
+        if (active && tid + i * team < nvec) emit(tid + i * team, y[i], m[i], ci);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < MAXV; ++i)
+        finish(tid + i * team, y[i], group_max(max_of(y[i], 0.f)));
+    }
     // uniform trip count: the shuffles need all lanes
     for (int v = tid + MAXV * team; v - tid < nvec; v += team) {
       F f;
@@ -436,6 +503,8 @@ extern "C" int to_add_rms_norm_group_quant(
   a.eps = eps;
   a.quant_eps = quant_eps;
   a.qmax = q_dtype == TO_E4M3 ? 448.0f : 127.0f;
+  a.qmax_inv = 1.0f / a.qmax;
+  a.cols_inv = 1.0f / (float)cols;
   a.floor_factor = a.qmax / quant_eps;
   a.ue8m0 = ue8m0;
   a.sl = ScaleLayout{column_major ? rows : 0, column_major ? cols / group_size : 1};
