@@ -306,7 +306,15 @@ TO_API int to_gemm(const void* a, const void* b, void* c, int dtype, int64_t M, 
 #define TO_EPI_GELU 3 /* tanh form */
 TO_API int to_gemm_bias_act(const void* a, int64_t lda, const void* b, const void* bias, int act,
                             const void* residual, int64_t ldr, void* c, int64_t ldc, int dtype,
-                            int64_t M, int64_t N, int64_t K, void* stream);
+                            int64_t M, int64_t N, int64_t K, void* workspace,
+                            size_t workspace_bytes, void* stream);
+/* Scratch for padded copies of operands whose rows are not 16-byte aligned (0 for aligned ones and
+ * for 128 tokens or fewer). It is optional: without it such a product runs on tiles that realign
+ * the operands as they read them, several times slower at many tokens. */
+TO_API size_t to_gemm_bias_act_workspace_size(const void* a, int64_t lda, const void* b, int dtype,
+                                              int64_t M, int64_t N, int64_t K);
+TO_API size_t to_w8a8_gemm_bias_act_workspace_size(const void* a, const void* b, int64_t M,
+                                                   int64_t N, int64_t K, int64_t block_k);
 /* Library extension: the W8A8 products with the same epilogue, C = act(sum_kb (A_kb B_kb^T)[m,n]
  * a_s[m,kb] b_s[n/block_n,kb] + bias) + residual. Operands and scales as to_w8a8_i8_gemm /
  * to_w8a8_fp8_gemm; bias, residual and C of c_dtype. One rounding (to_w8a8_*_gemm with a bias
@@ -316,12 +324,14 @@ TO_API int to_w8a8_i8_gemm_bias_act(const int8_t* a, const int8_t* b, const floa
                                     const float* b_s, const void* bias, int act,
                                     const void* residual, int64_t ldr, void* c, int64_t ldc,
                                     int c_dtype, int64_t M, int64_t N, int64_t K, int64_t block_n,
-                                    int64_t block_k, void* stream);
+                                    int64_t block_k, void* workspace, size_t workspace_bytes,
+                                    void* stream);
 TO_API int to_w8a8_fp8_gemm_bias_act(const void* a, const void* b, const float* a_s,
                                      const float* b_s, const void* bias, int act,
                                      const void* residual, int64_t ldr, void* c, int64_t ldc,
                                      int c_dtype, int64_t M, int64_t N, int64_t K, int64_t block_n,
-                                     int64_t block_k, void* stream);
+                                     int64_t block_k, void* workspace, size_t workspace_bytes,
+                                     void* stream);
 /* replaces tileops/blas/gemv.py:22 gemv (and its mv alias, :60): y [M] = A [M,K] @ x [K], A
  * row-major, dtype F32, F16 or BF16 for A, x and y, fp32 accumulation, y rounded once. Any M, K
  * (K = 0 writes zeros); 16-byte loads when K * sizeof(dtype) % 16 == 0 and A, x are 16-byte

@@ -89,7 +89,7 @@ def test_c_entries_check_before_they_launch():
     f16 = _lib.DTYPE_CODES[torch.float16]
 
     def gemm(m, n, k, act=0, dtype=f16, lda=8, ldr=8, ldc=8, p=1 << 20):
-        return lib.to_gemm_bias_act(p, lda, p, None, act, None, ldr, p, ldc, dtype, m, n, k, None)
+        return lib.to_gemm_bias_act(p, lda, p, None, act, None, ldr, p, ldc, dtype, m, n, k, None, 0, None)
 
     assert gemm(-1, 4, 4) == _lib.TO_EINVAL
     assert gemm(0, 4, 4) == _lib.TO_OK and gemm(4, 0, 4) == _lib.TO_OK
@@ -99,7 +99,7 @@ def test_c_entries_check_before_they_launch():
     assert gemm(2, 8, 8, p=None) == _lib.TO_EINVAL
     for fn in (lib.to_w8a8_i8_gemm_bias_act, lib.to_w8a8_fp8_gemm_bias_act):
         def w8a8(m, n, k, bn=1, bk=8, act=0, p=1 << 20, fn=fn):
-            return fn(p, p, p, p, None, act, None, n, p, n, f16, m, n, k, bn, bk, None)
+            return fn(p, p, p, p, None, act, None, n, p, n, f16, m, n, k, bn, bk, None, 0, None)
 
         assert w8a8(2, 2, 0) == _lib.TO_EINVAL and w8a8(2, 2, 8, bk=0) == _lib.TO_EINVAL
         assert w8a8(0, 2, 8) == _lib.TO_OK

@@ -14,6 +14,7 @@ import pytest
 import torch
 
 import tileops_b200 as tob
+from tileops_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -353,6 +354,77 @@ def test_offsets_past_32_bits(cuda):
         want = (k * a[rows, :1].float() * b[:1].float()
                 + (torch.arange(n, device=cuda) % 3).float()).bfloat16()
         assert torch.equal(y[rows], want)
+
+
+# Many tokens, nothing aligned: operands copied to aligned rows, outputs written row by row.
+RAGGED_SHAPES = [(129, 4097, 65), (200, 3001, 1000), (300, 9001, 777), (777, 2049, 1531),
+                 (513, 5003, 72), (1025, 1030, 33)]
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", RAGGED_SHAPES)
+def test_dense_exact_many_tokens_ragged(cuda, dt, m, n, k):
+    gen = torch.Generator(device=cuda).manual_seed(m + n + k)
+
+    def ri(lo, hi, *shape):
+        return torch.randint(lo, hi + 1, shape, generator=gen, device=cuda).to(dt)
+
+    a, b, bias, res = ri(-3, 3, m, k), ri(-2, 2, k, n), ri(-8, 8, n), ri(-8, 8, m, n)
+    want = exact_dense(a, b, bias, "relu", res).to(dt)
+    assert torch.equal(tob.gemm_bias_act(a, b, bias, act="relu", residual=res), want)
+    out = res.clone()
+    assert tob.gemm_bias_act(a, b, bias, act="relu", residual=out, out=out) is out
+    assert torch.equal(out, want)
+    # only A, only B off alignment; an aligned product into unaligned rows
+    flat = torch.zeros(m * k + 1, dtype=dt, device=cuda)
+    flat[1:] = a.reshape(-1)
+    assert torch.equal(tob.gemm_bias_act(flat[1:].view(m, k), b), exact_dense(a, b, None, None, None).to(dt))
+    k8, n8 = k // 8 * 8, n // 8 * 8
+    wide = torch.full((m, n8 + 3), 7, dtype=dt, device=cuda)
+    tob.gemm_bias_act(a[:, :k8].contiguous(), b[:k8, :n8].contiguous(), out=wide[:, 1:n8 + 1])
+    assert torch.equal(wide[:, 1:n8 + 1], exact_dense(a[:, :k8], b[:k8, :n8], None, None, None).to(dt))
+    assert bool((wide[:, 0] == 7).all()) and bool((wide[:, n8 + 1:] == 7).all())
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("scales", ["channel", "block128"])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", RAGGED_SHAPES)
+def test_w8a8_exact_many_tokens_ragged(cuda, codes, scales, dt, m, n, k):
+    gen = torch.Generator(device=cuda).manual_seed(m + n + k)
+    bn, bk = (1, k) if scales == "channel" else (128, 128)
+    hi, hi_b = (127, 3) if codes == "int8" else (8, 8)
+    cast = torch.int8 if codes == "int8" else torch.float8_e4m3fn
+
+    def ri(lo, hi, *shape):
+        return torch.randint(lo, hi + 1, shape, generator=gen, device=cuda).float()
+
+    a, b = ri(-hi, hi, m, k).to(cast), ri(-hi_b, hi_b, n, k).to(cast)
+    a_s, b_s = torch.exp2(ri(-1, 0, m, -(-k // bk))), torch.exp2(ri(-1, 0, -(-n // bn), -(-k // bk)))
+    bias, res = ri(-8, 8, n).to(dt), ri(-8, 8, m, n).to(dt)
+    op = (tob.w8a8_block_int8_matmul_bias_act if codes == "int8"
+          else tob.w8a8_block_fp8_matmul_bias_act)
+    y = op(a, b, a_s, b_s, [bn, bk], bias, act="relu", residual=res, output_dtype=dt)
+    assert torch.equal(y, w8a8_exact(a, b, a_s, b_s, bn, bk, bias, "relu", res).to(dt))
+
+
+def test_without_workspace(cuda):
+    """The C entry without scratch for copies: the same product on tiles that realign as they read."""
+    m, n, k = 300, 1001, 333
+    gen = torch.Generator(device=cuda).manual_seed(5)
+    a = torch.randint(-3, 4, (m, k), generator=gen, device=cuda).half()
+    b = torch.randint(-2, 3, (k, n), generator=gen, device=cuda).half()
+    c = torch.empty(m, n, device=cuda, dtype=torch.float16)
+    lib = _lib.load()
+    f16 = _lib.DTYPE_CODES[torch.float16]
+    assert lib.to_gemm_bias_act_workspace_size(a.data_ptr(), k, b.data_ptr(), f16, m, n, k) > 0
+    assert lib.to_gemm_bias_act_workspace_size(a.data_ptr(), k, b.data_ptr(), f16, 128, n, k) == 0
+    for ws in (0, 1024):
+        buf = torch.empty(max(ws, 1), dtype=torch.uint8, device=cuda)
+        c.zero_()
+        _lib.call("to_gemm_bias_act", a.data_ptr(), k, b.data_ptr(), None, 0, None, n, c.data_ptr(),
+                  n, f16, m, n, k, buf.data_ptr() if ws else None, ws, _lib.stream_ptr())
+        assert torch.equal(c, exact_dense(a, b, None, None, None).half())
 
 
 # Many tokens: several tiles per CTA pair, ragged last tiles, K of one slice, of an odd number of

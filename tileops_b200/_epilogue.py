@@ -67,6 +67,15 @@ def prepare(shape: tuple, n: int, like: torch.Tensor, dtype: torch.dtype,
     return bias, residual, ldr, like.new_empty(shape, dtype=dtype), n
 
 
+def copies(nbytes: int, like: torch.Tensor) -> tuple[Optional[torch.Tensor], Optional[int]]:
+    """Scratch for aligned copies of operands, allocated for this call alone: it can be as large as
+    the weights."""
+    if nbytes == 0:
+        return None, None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    return ws, ws.data_ptr()
+
+
 def finish(dst: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
     if out is not None and dst is not out:
         out.copy_(dst)
@@ -74,4 +83,4 @@ def finish(dst: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
     return dst
 
 
-__all__ = ["ACT_CODES", "check", "finish", "prepare"]
+__all__ = ["ACT_CODES", "check", "copies", "finish", "prepare"]

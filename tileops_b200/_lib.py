@@ -89,11 +89,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "to_w8a8_i8_gemm": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _L, _L, _L, _L, _L, _P]),
     "to_w8a8_fp8_gemm": (_I, [_P, _P, _P, _P, _P, _I, _P, _L, _L, _L, _L, _L, _P]),
     "to_gemm": (_I, [_P, _P, _P, _I, _L, _L, _L, _P]),
-    "to_gemm_bias_act": (_I, [_P, _L, _P, _P, _I, _P, _L, _P, _L, _I, _L, _L, _L, _P]),
+    "to_gemm_bias_act": (_I, [_P, _L, _P, _P, _I, _P, _L, _P, _L, _I, _L, _L, _L, _P, _S, _P]),
+    "to_gemm_bias_act_workspace_size": (_S, [_P, _L, _P, _I, _L, _L, _L]),
+    "to_w8a8_gemm_bias_act_workspace_size": (_S, [_P, _P, _L, _L, _L, _L]),
     "to_w8a8_i8_gemm_bias_act": (_I, [_P, _P, _P, _P, _P, _I, _P, _L, _P, _L, _I, _L, _L, _L, _L,
-                                      _L, _P]),
+                                      _L, _P, _S, _P]),
     "to_w8a8_fp8_gemm_bias_act": (_I, [_P, _P, _P, _P, _P, _I, _P, _L, _P, _L, _I, _L, _L, _L, _L,
-                                       _L, _P]),
+                                       _L, _P, _S, _P]),
     "to_gemv": (_I, [_P, _P, _P, _I, _L, _L, _P]),
     "to_silu_and_mul": (_I, [_P, _P, _P, _I, _L, _L, _L, _L, _L, _P]),
     "to_gelu_and_mul": (_I, [_P, _P, _P, _I, _L, _L, _L, _L, _L, _P]),

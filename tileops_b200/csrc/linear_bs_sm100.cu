@@ -1,5 +1,5 @@
 // W8A8 products with block scales and with bias, activation and residual in their epilogue, many
-// tokens: persistent 128 x BN tiles, one CTA per SM, 16-bit output.
+// tokens: persistent 128 x BN tiles, one CTA per SM.
 //   C = act( sum_kb (A_kb B_kb^T)[m, n] a_s[m, kb] b_s[n / bn, kb] + bias ) + residual
 //
 // The products of one 128-byte K slice land in one of two TMEM buffers of BN columns; eight
@@ -50,6 +50,7 @@ struct BsTile {
 
 struct BsArgs {
   int M, N, K, band;
+  int plain_out;  // output or residual is no TMA tensor
   LinEpi ep;
 };
 
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(kThreadsB, 1)
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
     prefetch_tmap(&tmC);
-    if (ep.res != nullptr) prefetch_tmap(&tmR);
+    if (ep.res != nullptr && !g.plain_out) prefetch_tmap(&tmR);
     if (misaligned && err) atomicExch(err, (int)kErrSmemAlign);
   }
   if (warp == 1) tmem_alloc<512>(tmem_holder);
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(kThreadsB, 1)
     const int c_first = eg * kMax;                                 // this warp's first chunk
     const int c_count = eg == 0 ? kMax : kChunks - kMax;
     ChunkWriter wr{slabs + ew * 2 * kSlab, rbar + 2 * ew, &tmC, &tmR, abort_flag, err,
-                   ep.form, ep.dtype, lane, ep.res != nullptr};
+                   ep.form, ep.dtype, lane, ep.res != nullptr && !g.plain_out};
     grid_dependency_wait();
     int fill = 0, blk = 0;  // buffers folded, blocks of scales used
     bool ok = true;
@@ -340,9 +341,13 @@ __global__ void __launch_bounds__(kThreadsB, 1)
 #pragma unroll 1
       for (int j = 0; j < mine; ++j) {
         const int c0 = (c_first + j) * 32;
-        if (!wr.acquire()) ok = false;
-        wr.put(run, bias + c0, n0 + c0, row0, ok);
-        if (j + 2 < mine) wr.fetch(1, n0 + c0 + 64, row0);
+        if (g.plain_out) {
+          wr.put_plain(run, bias + c0, n0 + c0, row0, ep, g.M, g.N, ok);
+        } else {
+          if (!wr.acquire()) ok = false;
+          wr.put(run, bias + c0, n0 + c0, row0, ok);
+          if (j + 2 < mine) wr.fetch(1, n0 + c0 + 64, row0);
+        }
 #pragma unroll
         for (int i = 0; i < (kMax - 1) * 32; ++i) run[i] = run[i + 32];
       }
@@ -366,14 +371,15 @@ __global__ void __launch_bounds__(kThreadsB, 1)
 }
 
 template <Kind KD, int BN>
-int launch_bs(const void* a, int64_t lda, const void* b, int64_t M, int64_t N, int64_t K,
-              const LinEpi& ep, cudaStream_t st) {
+int launch_bs(const LinOps& o, bool plain_out, const LinEpi& ep, cudaStream_t st) {
   using C = BsTile<BN>;
   auto kern = k_linear_bs<KD, BN>;
   const cudaError_t ae = ensure_smem_attr((const void*)kern, (int)C::kSmem);
   if (ae != cudaSuccess) return cuda_fail(ae, "linear epilogue (block scales): shared memory");
+  const int64_t M = o.M, N = o.N, K = o.K;
   BsArgs g;
   memset((void*)&g, 0, sizeof(g));
+  g.plain_out = plain_out;
   g.M = (int)M;
   g.N = (int)N;
   g.K = (int)K;
@@ -381,11 +387,12 @@ int launch_bs(const void* a, int64_t lda, const void* b, int64_t M, int64_t N, i
   g.band = (int64_t)32 * 128 * K <= ((int64_t)32 << 20) ? 32 : 16;
   g.ep = ep;
   CUtensorMap ta, tb, tc, tr;
+  memset(&tc, 0, sizeof(tc));
   memset(&tr, 0, sizeof(tr));
-  int rc = kmajor_map(&ta, a, M, K, lda, 1, 128, 1);
-  if (!rc) rc = kmajor_map(&tb, b, N, K, K, 1, BN, 1);
-  if (!rc) rc = chunk_map(&tc, ep.c, M, N, ep.ldc);
-  if (!rc && ep.res != nullptr) rc = chunk_map(&tr, ep.res, M, N, ep.ldr);
+  int rc = kmajor_map(&ta, o.a, M, o.a_k, o.lda, 1, 128, 1);
+  if (!rc) rc = kmajor_map(&tb, o.b, N, o.b_in, o.ldb, 1, BN, 1);
+  if (!rc && !plain_out) rc = chunk_map(&tc, ep.c, M, N, ep.ldc);
+  if (!rc && !plain_out && ep.res != nullptr) rc = chunk_map(&tr, ep.res, M, N, ep.ldr);
   if (rc) return rc;
   const int64_t tiles = ceil_div(M, 128) * ceil_div(N, BN);
   cudaLaunchConfig_t cfg = {};
@@ -405,18 +412,12 @@ int launch_bs(const void* a, int64_t lda, const void* b, int64_t M, int64_t N, i
 
 }  // namespace
 
-// Runs a block-scaled product on 128 x BN tiles, or returns TO_EUNSUPPORTED (nothing launched)
-// where they do not apply: 16-bit output, rows of every operand 16-byte aligned, column blocks that
-// are whole 32-column chunks, and enough tiles to fill the SMs.
-int linear_bs_launch(int kind, const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
-                     int64_t K, const LinEpi& ep, cudaStream_t st) {
-  if (M <= 64 || (ep.dtype != TO_F16 && ep.dtype != TO_BF16)) return TO_EUNSUPPORTED;
-  if (!aligned_rows(a, lda) || !aligned_rows(b, K) || !aligned_rows(ep.c, ep.ldc * 2) ||
-      (ep.res && !aligned_rows(ep.res, ep.ldr * 2)))
-    return TO_EUNSUPPORTED;
-  if (ep.bn % 32 != 0 && ep.bn < N) return TO_EUNSUPPORTED;
-  // Tile width: the one whose rounds of tiles cost least; a tile's time is its width plus a fixed
-  // part worth about 32 columns.
+// The tile width for a block-scaled product, 0 where these tiles do not pay or apply: column blocks
+// have to be whole 32-column chunks, and the tiles to fill the SMs.
+int linear_bs_width(int64_t M, int64_t N, int64_t bn) {
+  if (M <= 64 || (bn % 32 != 0 && bn < N)) return 0;
+  // The width whose rounds of tiles cost least; a tile's time is its width plus a fixed part worth
+  // about 32 columns.
   const int64_t mt = ceil_div(M, 128), sms = sm_count();
   int best = 0;
   int64_t best_cost = 0;
@@ -428,14 +429,22 @@ int linear_bs_launch(int kind, const void* a, int64_t lda, const void* b, int64_
       best_cost = cost;
     }
   }
-  if (mt * ceil_div(N, best) > INT32_MAX) return TO_EUNSUPPORTED;
-  if (mt * ceil_div(N, best) * 2 < sms) return TO_EUNSUPPORTED;  // split K instead
+  const int64_t tiles = mt * ceil_div(N, best);
+  return tiles > INT32_MAX || tiles * 2 < sms ? 0 : best;  // few tiles: split K instead
+}
+
+// Runs it, or returns TO_EUNSUPPORTED (nothing launched, nothing recorded). Rows of A and B have to
+// be 16-byte aligned.
+int linear_bs_launch(int kind, const LinOps& o, const LinEpi& ep, cudaStream_t st) {
+  const int best = linear_bs_width(o.M, o.N, ep.bn);
+  if (best == 0 || !aligned_rows(o.a, o.lda) || !aligned_rows(o.b, o.ldb)) return TO_EUNSUPPORTED;
+  const bool plain = plain_output(ep);
   auto run = [&](auto kd) {
     constexpr Kind KD = decltype(kd)::value;
     switch (best) {
-      case 224: return launch_bs<KD, 224>(a, lda, b, M, N, K, ep, st);
-      case 192: return launch_bs<KD, 192>(a, lda, b, M, N, K, ep, st);
-      default: return launch_bs<KD, 128>(a, lda, b, M, N, K, ep, st);
+      case 224: return launch_bs<KD, 224>(o, plain, ep, st);
+      case 192: return launch_bs<KD, 192>(o, plain, ep, st);
+      default: return launch_bs<KD, 128>(o, plain, ep, st);
     }
   };
   return kind == TO_I8 ? run(std::integral_constant<Kind, Kind::I8>{})

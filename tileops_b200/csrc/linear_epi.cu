@@ -7,11 +7,13 @@ namespace sm100 {
 int linear_nt_launch(int kind, bool block_scaled, const void* x, int64_t ldx, const void* w,
                      int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st);
 // TO_EUNSUPPORTED (nothing launched) where the tiles do not apply.
-int linear_pair_launch(int kind, const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
-                       int64_t K, const LinEpi& ep, cudaStream_t st);
-int linear_bs_launch(int kind, const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
-                     int64_t K, const LinEpi& ep, cudaStream_t st);
+int linear_pair_launch(int kind, const LinOps& o, const LinEpi& ep, cudaStream_t st);
+int linear_pair_width(int kind, int64_t M, int64_t N);
+int linear_bs_launch(int kind, const LinOps& o, const LinEpi& ep, cudaStream_t st);
+int linear_bs_width(int64_t M, int64_t N, int64_t bn);
 }
+int64_t linear_relay_bytes(int kind, const LinOps& o);
+int linear_relay(int kind, LinOps* o, void* ws, cudaStream_t st);
 int linear_dense_simt_launch(const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
                              int64_t K, const LinEpi& ep, cudaStream_t st);
 int linear_w8a8_simt_launch(bool fp8, const void* a, const void* b, int64_t M, int64_t N, int64_t K,
@@ -19,13 +21,39 @@ int linear_w8a8_simt_launch(bool fp8, const void* a, const void* b, int64_t M, i
 
 namespace {
 
-// Many tokens: CTA-pair tiles, or folding tiles with block scales; few tokens, a small grid or any misalignment: weights as rows.
-int tensor_core_launch(int kind, bool block_scaled, const void* a, int64_t lda, const void* b,
-                       int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st) {
-  const int rc = block_scaled ? sm100::linear_bs_launch(kind, a, lda, b, M, N, K, ep, st)
-                              : sm100::linear_pair_launch(kind, a, lda, b, M, N, K, ep, st);
+// Tokens from which a product is worth aligned copies of operands that TMA cannot read: below, one
+// column of tiles reads the weights once at any alignment; above, every further 128 tokens would
+// realign them again.
+constexpr int64_t kRelayTokens = 128;
+
+LinOps make_ops(const void* a, int64_t lda, const void* b, int64_t M, int64_t N, int64_t K,
+                bool b_mn) {
+  return LinOps{a, b, lda, b_mn ? N : K, K, b_mn ? N : K, M, N, K};
+}
+
+int64_t relay_bytes(int kind, const LinOps& o) {
+  return o.M > kRelayTokens ? linear_relay_bytes(kind, o) : 0;
+}
+
+// Many tokens: CTA-pair tiles, or folding tiles with block scales, over aligned copies where need be
+// and the caller's workspace allows; few tokens, a small grid, or no workspace: weights as rows.
+int tensor_core_launch(int kind, bool block_scaled, LinOps o, LinEpi ep, void* ws, size_t ws_bytes,
+                       cudaStream_t st) {
+  const LinOps given = o;
+  const bool tiles = (block_scaled ? sm100::linear_bs_width(o.M, o.N, ep.bn)
+                                   : sm100::linear_pair_width(kind, o.M, o.N)) != 0;
+  const int64_t need = tiles ? relay_bytes(kind, o) : 0;
+  if (need > 0 && ws != nullptr && (int64_t)ws_bytes >= need &&
+      (reinterpret_cast<uint64_t>(ws) & 15u) == 0) {
+    const int rc = linear_relay(kind, &o, ws, st);
+    if (rc) return rc;
+    ep.early_weights = 0;  // the copies are the previous kernel's output
+  }
+  const int rc = block_scaled ? sm100::linear_bs_launch(kind, o, ep, st)
+                              : sm100::linear_pair_launch(kind, o, ep, st);
   if (rc != TO_EUNSUPPORTED) return rc;
-  return sm100::linear_nt_launch(kind, block_scaled, a, lda, b, M, N, K, ep, st);
+  return sm100::linear_nt_launch(kind, block_scaled, given.a, given.lda, given.b, given.M, given.N,
+                                 given.K, ep, st);
 }
 
 // Fills the epilogue common to both products; TO_OK or a recorded failure.
@@ -55,7 +83,7 @@ int make_epi(LinEpi* ep, const char* op, const void* bias, int act, const void* 
 int w8a8_epi_entry(bool fp8, const void* a, const void* b, const float* a_s, const float* b_s,
                    const void* bias, int act, const void* res, int64_t ldr, void* c, int64_t ldc,
                    int c_dtype, int64_t M, int64_t N, int64_t K, int64_t bn, int64_t bk,
-                   void* stream) {
+                   void* ws, size_t ws_bytes, void* stream) {
   const char* op = fp8 ? "w8a8_block_fp8_matmul_bias_act" : "w8a8_block_int8_matmul_bias_act";
   if (M < 0 || N < 0 || K <= 0 || bn <= 0 || bk <= 0 || M > INT32_MAX || N > INT32_MAX ||
       K > INT32_MAX)
@@ -76,7 +104,8 @@ int w8a8_epi_entry(bool fp8, const void* a, const void* b, const float* a_s, con
   if (kt > 1 && bk % 128 != 0)
     return linear_w8a8_simt_launch(fp8, a, b, M, N, K, ep.bn, bk, ep, st);
   ep.kb_per_scale = kt > 1 ? (int)(bk / 128) : 1;
-  return tensor_core_launch(fp8 ? TO_E4M3 : TO_I8, kt > 1, a, K, b, M, N, K, ep, st);
+  return tensor_core_launch(fp8 ? TO_E4M3 : TO_I8, kt > 1, make_ops(a, K, b, M, N, K, false), ep,
+                            ws, ws_bytes, st);
 }
 
 }  // namespace
@@ -84,9 +113,21 @@ int w8a8_epi_entry(bool fp8, const void* a, const void* b, const float* a_s, con
 
 extern "C" {
 
+size_t to_gemm_bias_act_workspace_size(const void* a, int64_t lda, const void* b, int dtype,
+                                       int64_t M, int64_t N, int64_t K) {
+  if ((dtype != TO_F16 && dtype != TO_BF16) || M <= 0 || N <= 0 || K <= 0) return 0;
+  return (size_t)tob::relay_bytes(dtype, tob::make_ops(a, lda, b, M, N, K, true));
+}
+
+size_t to_w8a8_gemm_bias_act_workspace_size(const void* a, const void* b, int64_t M, int64_t N,
+                                            int64_t K, int64_t block_k) {
+  if (M <= 0 || N <= 0 || K <= 0 || block_k <= 0 || (block_k < K && block_k % 128 != 0)) return 0;
+  return (size_t)tob::relay_bytes(TO_I8, tob::make_ops(a, K, b, M, N, K, false));
+}
+
 int to_gemm_bias_act(const void* a, int64_t lda, const void* b, const void* bias, int act,
                      const void* residual, int64_t ldr, void* c, int64_t ldc, int dtype, int64_t M,
-                     int64_t N, int64_t K, void* stream) {
+                     int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace tob;
   const char* op = "gemm_bias_act";
   if (M < 0 || N < 0 || K < 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX)
@@ -103,23 +144,26 @@ int to_gemm_bias_act(const void* a, int64_t lda, const void* b, const void* bias
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == TO_F32 || K == 0)
     return linear_dense_simt_launch(a, lda, b, M, N, K, ep, st);
-  return tensor_core_launch(dtype, false, a, lda, b, M, N, K, ep, st);
+  return tensor_core_launch(dtype, false, make_ops(a, lda, b, M, N, K, true), ep, workspace,
+                            workspace_bytes, st);
 }
 
 int to_w8a8_i8_gemm_bias_act(const int8_t* a, const int8_t* b, const float* a_s, const float* b_s,
                              const void* bias, int act, const void* residual, int64_t ldr, void* c,
                              int64_t ldc, int c_dtype, int64_t M, int64_t N, int64_t K,
-                             int64_t block_n, int64_t block_k, void* stream) {
+                             int64_t block_n, int64_t block_k, void* workspace,
+                             size_t workspace_bytes, void* stream) {
   return tob::w8a8_epi_entry(false, a, b, a_s, b_s, bias, act, residual, ldr, c, ldc, c_dtype, M, N,
-                             K, block_n, block_k, stream);
+                             K, block_n, block_k, workspace, workspace_bytes, stream);
 }
 
 int to_w8a8_fp8_gemm_bias_act(const void* a, const void* b, const float* a_s, const float* b_s,
                               const void* bias, int act, const void* residual, int64_t ldr, void* c,
                               int64_t ldc, int c_dtype, int64_t M, int64_t N, int64_t K,
-                              int64_t block_n, int64_t block_k, void* stream) {
+                              int64_t block_n, int64_t block_k, void* workspace,
+                              size_t workspace_bytes, void* stream) {
   return tob::w8a8_epi_entry(true, a, b, a_s, b_s, bias, act, residual, ldr, c, ldc, c_dtype, M, N,
-                             K, block_n, block_k, stream);
+                             K, block_n, block_k, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

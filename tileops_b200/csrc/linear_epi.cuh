@@ -70,6 +70,16 @@ struct LinEpi {
   ActForm form = {};           // act_form(act)
 };
 
+// The operands of a product: A [M, K] rows lda elements apart, B [N, K] (8-bit) or [K, N] (16-bit)
+// rows ldb apart. a_k >= K: columns of A that exist, zero past K (a padded copy); b_in likewise for
+// the inner dimension of B.
+struct LinOps {
+  const void* a;
+  const void* b;
+  int64_t lda, ldb, a_k, b_in;
+  int64_t M, N, K;
+};
+
 // Element i of an array of `dtype` (TO_F32 / TO_F16 / TO_BF16) as fp32, and its store. The
 // residual may be the output itself (in-place add), so its loads stay ordinary loads.
 __device__ __forceinline__ float ld_dtype(const void* p, int64_t i, int dtype) {

@@ -13,8 +13,8 @@
 // distributed shared memory in rank order (deterministic, no workspace).
 //
 // Operands come by TMA when their rows are 16-byte aligned (PLAIN = false). Any other stride,
-// offset or size takes PLAIN: eight warps load the rows with the widest loads their alignment
-// allows, realign them in registers and store them in the same swizzled layout.
+// offset or size takes PLAIN: eight warps load the rows by aligned words, shift them together in
+// registers and store them in the same swizzled layout.
 //
 // Roles: warp 0 weight copies, warp 1 MMA issue and TMEM, warp 2 token copies, warp 3 idle, then
 // kEpiWarps epilogue warps (lane quarter = warp % 4) and, with PLAIN, kLoadWarps loaders.
@@ -24,8 +24,10 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "linear_epi.cuh"
+#include "realign.cuh"
 #include "sm100.cuh"
 
 namespace tob {
@@ -66,44 +68,8 @@ struct NtArgs {
   const uint8_t* w;
   const uint8_t* x;
   int64_t w_pitch, x_pitch;  // bytes between rows
-  int w_align, x_align;      // largest power of two <= 16 dividing base and pitch
   LinEpi ep;
 };
-
-// 16 bytes at p, of which the first `valid` (0..16) exist; the rest read as zero. `align` divides
-// p. [lo, hi) is the operand's memory: nothing outside it is touched.
-__device__ __forceinline__ uint4 load_chunk(const uint8_t* p, int valid, int align,
-                                            const uint8_t* lo, const uint8_t* hi) {
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-  if (valid >= 16 && align >= 4) {
-    if (align >= 16) return __ldg(reinterpret_cast<const uint4*>(p));
-    if (align == 8) {
-      const uint2 a = __ldg(reinterpret_cast<const uint2*>(p));
-      const uint2 b = __ldg(reinterpret_cast<const uint2*>(p) + 1);
-      return make_uint4(a.x, a.y, b.x, b.y);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
-  } else if (valid > 0) {
-    // Aligned words around p, shifted together. A word that would reach outside the operand, or
-    // past the row's valid bytes, is assembled from single bytes.
-    const int sh = (int)(reinterpret_cast<uintptr_t>(p) & 3u);
-    const uint8_t* base = p - sh;
-    if (valid >= 16 && base >= lo && base + 20 <= hi) {
-      uint32_t r[5];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = __ldg(reinterpret_cast<const uint32_t*>(base) + i);
-      r[4] = sh ? __ldg(reinterpret_cast<const uint32_t*>(base) + 4) : 0u;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(r[i], r[i + 1], 8 * sh);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < valid) w[i / 4] |= (uint32_t)__ldg(p + i) << (8 * (i % 4));
-    }
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
 
 template <Kind KD, int NT, bool BS, bool PLAIN>
 __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
@@ -253,46 +219,54 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
       const uint8_t* w_hi = g.w + (w_rows - 1) * g.w_pitch + w_bytes;
       const uint8_t* x_hi = g.x + (int64_t)(g.M - 1) * g.x_pitch + row_bytes;
       grid_dependency_wait();
+      constexpr int kBatch = 4;  // 16-byte pieces whose loads a lane has in flight
       for (int it = 0; it < kb_n; ++it) {
         const int s = it % ST;
         const int64_t kbyte = (int64_t)(kb_lo + it) * 128;
-        uint4 v[kMine];
-  #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const int row = (lw + i * C::kLoadWarps) * 4 + (lane >> 3);
-          v[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (row < 128) {
-            int64_t r, off;  // source row and byte offset in it
-            if (C::kMn) {
-              r = (int64_t)(kb_lo + it) * 64 + (row & 63);
-              off = (int64_t)(n0 + (row & 64)) * 2 + chunk * 16;
+        bool waited = it < ST;
+#pragma unroll
+        for (int i0 = 0; i0 < kMine; i0 += kBatch) {
+          Unaligned16 v[kBatch];
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const int row = (lw + (i0 + i) * C::kLoadWarps) * 4 + (lane >> 3);
+            if (row < 128) {
+              int64_t r, off;  // source row and byte offset in it
+              if (C::kMn) {
+                r = (int64_t)(kb_lo + it) * 64 + (row & 63);
+                off = (int64_t)(n0 + (row & 64)) * 2 + chunk * 16;
+              } else {
+                r = n0 + row;
+                off = kbyte + chunk * 16;
+              }
+              const int64_t left = r < w_rows ? w_bytes - off : 0;
+              v[i].issue(g.w + r * g.w_pitch + off, (int)max((int64_t)0, min((int64_t)16, left)),
+                         g.w, w_hi);
             } else {
-              r = n0 + row;
-              off = kbyte + chunk * 16;
+              const int t = row - 128;
+              const int64_t off = kbyte + chunk * 16;
+              const int64_t left = t < tokens ? row_bytes - off : 0;
+              v[i].issue(g.x + (int64_t)(t0 + t) * g.x_pitch + off,
+                         (int)max((int64_t)0, min((int64_t)16, left)), g.x, x_hi);
             }
-            if (r < w_rows && off < w_bytes)
-              v[i] = load_chunk(g.w + r * g.w_pitch + off, (int)min((int64_t)16, w_bytes - off),
-                                g.w_align, g.w, w_hi);
-          } else if (row < 128 + NT) {
-            const int t = row - 128;
-            const int64_t off = kbyte + chunk * 16;
-            if (t < tokens && off < row_bytes)
-              v[i] = load_chunk(g.x + (int64_t)(t0 + t) * g.x_pitch + off,
-                                (int)min((int64_t)16, row_bytes - off), g.x_align, g.x, x_hi);
+          }
+          if (!waited) {
+            if (!mbar_wait_polled(empty + s, ((uint32_t)(it / ST) & 1u) ^ 1, abort_flag, err)) {
+              ok = false;
+              break;
+            }
+            waited = true;
+          }
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const int row = (lw + (i0 + i) * C::kLoadWarps) * 4 + (lane >> 3);
+            if (row >= 128 + NT) continue;
+            uint8_t* tile = row < 128 ? sW + (size_t)s * C::kWBytes : sX + (size_t)s * C::kXBytes;
+            const int r = row < 128 ? row : row - 128;
+            *reinterpret_cast<uint4*>(tile + r * 128 + ((chunk ^ (r & 7)) << 4)) = v[i].finish();
           }
         }
-        if (it >= ST && !mbar_wait_polled(empty + s, ((uint32_t)(it / ST) & 1u) ^ 1, abort_flag, err)) {
-          ok = false;
-          break;
-        }
-  #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const int row = (lw + i * C::kLoadWarps) * 4 + (lane >> 3);
-          if (row >= 128 + NT) continue;
-          uint8_t* tile = row < 128 ? sW + (size_t)s * C::kWBytes : sX + (size_t)s * C::kXBytes;
-          const int r = row < 128 ? row : row - 128;
-          *reinterpret_cast<uint4*>(tile + r * 128 + ((chunk ^ (r & 7)) << 4)) = v[i];
-        }
+        if (!ok) break;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(full + s);
@@ -380,50 +354,55 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
   // every thread reads back its own tokens, so no barrier is needed.
   if (S > 1) cluster_sync_all();
   if (epi && ok && n_ok) {
-    const uint32_t mine = smem_u32(part + q * 32 + lane);
-    const int step = S > 1 ? S * (C::kEpiWarps / 4) : 1;
-    const int first = S > 1 ? rank + half * S : half * C::kTpt;
-    const int last = S > 1 ? tokens : min(tokens, (half + 1) * C::kTpt);
-    constexpr int U = 2;  // tokens whose loads are in flight together
+    // Tokens whose loads are in flight together (U) and partial sums per token (P).
+    auto tokens_loop = [&](auto u_tag, auto p_tag, int first, int last, int step) {
+      constexpr int U = decltype(u_tag)::value, P = decltype(p_tag)::value;
+      const uint32_t mine = smem_u32(part + q * 32 + lane);
 #pragma unroll 1
-    for (int tok = first; tok < last; tok += U * step) {
-      float res[U], sc[U];
-      uint32_t v[U][8];
+      for (int tok = first; tok < last; tok += U * step) {
+        float res[U], sc[U];
+        uint32_t v[U][P];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = min(tok + u * step, last - 1);
-        if (S > 1) {
+        for (int u = 0; u < U; ++u) {
+          const int t = min(tok + u * step, last - 1);
+          if constexpr (P > 1) {
 #pragma unroll
-          for (int s = 0; s < 8; ++s) {
-            v[u][s] = 0u;
-            if (s < S)
-              asm volatile("ld.shared::cluster.u32 %0, [%1];"
-                           : "=r"(v[u][s])
-                           : "r"(mapa_shared(mine + (uint32_t)t * 512u, (uint32_t)s))
-                           : "memory");
+            for (int s = 0; s < P; ++s) {
+              v[u][s] = 0u;
+              if (s < S)
+                asm volatile("ld.shared::cluster.u32 %0, [%1];"
+                             : "=r"(v[u][s])
+                             : "r"(mapa_shared(mine + (uint32_t)t * 512u, (uint32_t)s))
+                             : "memory");
+            }
+          } else {
+            v[u][0] = reinterpret_cast<const uint32_t*>(part)[t * 128 + q * 32 + lane];
           }
-        } else {
-          v[u][0] = reinterpret_cast<const uint32_t*>(part)[t * 128 + q * 32 + lane];
+          res[u] = ep.res != nullptr ? ld_dtype(ep.res, (int64_t)(t0 + t) * ep.ldr + n, ep.dtype)
+                                     : 0.f;
+          sc[u] = 1.f;
+          if (!BS && ep.a_s != nullptr)
+            sc[u] = __ldg(ep.a_s + (int64_t)(t0 + t) * ep.a_s_ld) * sb;
         }
-        res[u] = ep.res != nullptr ? ld_dtype(ep.res, (int64_t)(t0 + t) * ep.ldr + n, ep.dtype)
-                                   : 0.f;
-        sc[u] = 1.f;
-        if (!BS && ep.a_s != nullptr) sc[u] = __ldg(ep.a_s + (int64_t)(t0 + t) * ep.a_s_ld) * sb;
-      }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        uint32_t sum = v[u][0];
-        if (S > 1) {
+        for (int u = 0; u < U; ++u) {
+          uint32_t sum = v[u][0];
 #pragma unroll
-          for (int s = 1; s < 8; ++s) {
+          for (int s = 1; s < P; ++s) {
             if (KD == Kind::I8 && !BS) sum += v[u][s];
             else if (s < S) sum = __float_as_uint(__uint_as_float(sum) + __uint_as_float(v[u][s]));
           }
+          const float acc = KD == Kind::I8 && !BS ? (float)(int32_t)sum : __uint_as_float(sum);
+          if (tok + u * step < last) finish(acc * sc[u], tok + u * step, res[u]);
         }
-        const float acc = KD == Kind::I8 && !BS ? (float)(int32_t)sum : __uint_as_float(sum);
-        if (tok + u * step < last) finish(acc * sc[u], tok + u * step, res[u]);
       }
-    }
+    };
+    if (S > 1)
+      tokens_loop(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{},
+                  rank + half * S, tokens, S * (C::kEpiWarps / 4));
+    else
+      tokens_loop(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{},
+                  half * C::kTpt, min(tokens, (half + 1) * C::kTpt), 1);
   }
   grid_dependency_wait();
   tc_fence_before();
@@ -507,8 +486,6 @@ int launch_nt(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, i
   g.x = (const uint8_t*)x;
   g.w_pitch = (C::kMn ? N : K) * C::kElem;
   g.x_pitch = ldx * C::kElem;
-  g.w_align = pow2_align(w, g.w_pitch);
-  g.x_align = pow2_align(x, g.x_pitch);
   g.ep = ep;
   CUtensorMap tw, tx;
   memset(&tw, 0, sizeof(tw));

@@ -1,5 +1,5 @@
 // Products with bias, activation and residual in their epilogue, many tokens: 256 x BN output tiles
-// on CTA pairs (tcgen05 cta_group::2), persistent over the tiles, 16-bit output.
+// on CTA pairs (tcgen05 cta_group::2), persistent over the tiles.
 //
 //   A tokens [M, K] (K-major); B weights int8 / e4m3 [N, K] (K-major) or fp16 / bf16 [K, N]
 //   (MN-major, 64-column strips)
@@ -51,8 +51,9 @@ struct PairCfg2 {
 
 struct PairArgs {
   int M, N, K;
-  int slices3d;    // K-major operands through {128 B, rows, slices} maps (K is whole slices)
-  int strips3d;    // MN-major B through the strip map (N % 64 == 0)
+  int a3d, b3d;    // operand through a 3-D map: {128 B, rows, slices} of whole slices, or (MN-major
+                   // B) {64 columns, K rows, strips} of whole strips
+  int plain_out;   // output or residual is no TMA tensor
   int band;        // M tiles per band of the tile order
   int small_m;     // one row of tiles: A stays in L2, B streams
   LinEpi ep;
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(kThreadsP, 1)
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
     prefetch_tmap(&tmC);
-    if (ep.res != nullptr) prefetch_tmap(&tmR);
+    if (ep.res != nullptr && !g.plain_out) prefetch_tmap(&tmR);
     if (misaligned && err) atomicExch(err, (int)kErrSmemAlign);
   }
   cluster_arrive_relaxed();
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(kThreadsP, 1)
               issued_phase = (issued_phase & ~(1u << s)) | (ph << s);
             }
             uint8_t* dst = sA + (size_t)s * C::kABytes;
-            if (g.slices3d) {
+            if (g.a3d) {
               tma_load_3d_pair(dst, &tmA, 0, arow, sl, bar, pol);
             } else {
 #pragma unroll
@@ -163,14 +164,14 @@ __global__ void __launch_bounds__(kThreadsP, 1)
             uint8_t* dst = sB + (size_t)s * C::kBBytes;
             if constexpr (C::kMn) {
               // strips of 128 K rows x 64 columns, 16 KB each
-              if (g.strips3d) {
+              if (g.b3d) {
                 tma_load_3d_pair(dst, &tmB, 0, k, bcol / 64, bar, pol);
               } else {
 #pragma unroll
                 for (int c = 0; c < BN / 128; ++c)
                   tma_load_2d_pair(dst + c * 16384, &tmB, bcol + 64 * c, k, bar, pol);
               }
-            } else if (g.slices3d) {
+            } else if (g.b3d) {
               tma_load_3d_pair(dst, &tmB, 0, bcol, sl, bar, pol);
             } else {
 #pragma unroll
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(kThreadsP, 1)
     constexpr int kMine = (kChunks + 1) / 2;
     const uint32_t lead_tempty = mapa_shared(smem_u32(tempty), 0);
     ChunkWriter wr{slabs + ew * 2 * kSlab, rbar + 2 * ew, &tmC, &tmR, abort_flag, err,
-                   ep.form, ep.dtype, lane, ep.res != nullptr};
+                   ep.form, ep.dtype, lane, ep.res != nullptr && !g.plain_out};
     grid_dependency_wait();
     int fill = 0;  // accumulator fills read
     bool ok = true;
@@ -313,6 +314,10 @@ __global__ void __launch_bounds__(kThreadsP, 1)
             v[i + u] = C::kMn ? a : a * (sa * sbv[u]);
           }
         }
+        if (g.plain_out) {
+          wr.put_plain(v, bias + c0, n0 + c0, row0, ep, g.M, g.N, ok);
+          continue;
+        }
         if (!wr.acquire()) ok = false;
         wr.put(v, bias + c0, n0 + c0, row0, ok);
         if (j + 2 < mine) wr.fetch(1, n0 + chunk_col(j + 2), row0);
@@ -341,45 +346,46 @@ __global__ void __launch_bounds__(kThreadsP, 1)
 }
 
 template <Kind KD, int BN>
-int launch_pair(const void* a, int64_t lda, const void* b, int64_t M, int64_t N, int64_t K,
-                const LinEpi& ep, cudaStream_t st) {
+int launch_pair(const LinOps& o, bool plain_out, const LinEpi& ep, cudaStream_t st) {
   using C = PairCfg2<KD, BN>;
   auto kern = k_linear_pair<KD, BN>;
   const cudaError_t ae = ensure_smem_attr((const void*)kern, (int)C::kSmem);
   if (ae != cudaSuccess) return cuda_fail(ae, "linear epilogue (pairs): shared memory attribute");
+  const int64_t M = o.M, N = o.N, K = o.K;
   PairArgs g;
   memset((void*)&g, 0, sizeof(g));
   g.M = (int)M;
   g.N = (int)N;
   g.K = (int)K;
-  g.slices3d = (K * C::kElem) % 128 == 0;
-  g.strips3d = C::kMn && N % 64 == 0;
+  g.a3d = (o.a_k * C::kElem) % 128 == 0;
+  g.b3d = (o.b_in * C::kElem) % 128 == 0;
+  g.plain_out = plain_out;
   // Bands whose A rows stay within 32 MB of L2.
   g.band = (int64_t)16 * 256 * K * C::kElem <= ((int64_t)32 << 20) ? 16 : 8;
   g.small_m = M <= 256;
   g.ep = ep;
   CUtensorMap ta, tb, tc, tr;
+  memset(&tc, 0, sizeof(tc));
   memset(&tr, 0, sizeof(tr));
-  int rc = kmajor_map(&ta, a, M, K, lda * C::kElem, C::kElem, 128, g.slices3d ? kKC : 1);
+  int rc = kmajor_map(&ta, o.a, M, o.a_k, o.lda * C::kElem, C::kElem, 128, g.a3d ? kKC : 1);
   if (rc) return rc;
   if (!C::kMn) {
-    rc = kmajor_map(&tb, b, N, K, K * C::kElem, C::kElem, BN / 2, g.slices3d ? kKC : 1);
-  } else if (g.strips3d) {
-    const cuuint64_t dims[3] = {64, (cuuint64_t)K, (cuuint64_t)(N / 64)};
-    const cuuint64_t strides[2] = {(cuuint64_t)(N * 2), 128};
+    rc = kmajor_map(&tb, o.b, N, o.b_in, o.ldb, C::kElem, BN / 2, g.b3d ? kKC : 1);
+  } else if (g.b3d) {
+    const cuuint64_t dims[3] = {64, (cuuint64_t)K, (cuuint64_t)(o.b_in / 64)};
+    const cuuint64_t strides[2] = {(cuuint64_t)(o.ldb * 2), 128};
     const cuuint32_t box[3] = {64, 64 * kKC, BN / 128};
-    rc = tiled_map(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT16, b, 3, dims, strides, box,
+    rc = tiled_map(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT16, o.b, 3, dims, strides, box,
                    CU_TENSOR_MAP_SWIZZLE_128B);
   } else {
-    const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)K};
-    const cuuint64_t strides[1] = {(cuuint64_t)(N * 2)};
+    const cuuint64_t dims[2] = {(cuuint64_t)o.b_in, (cuuint64_t)K};
+    const cuuint64_t strides[1] = {(cuuint64_t)(o.ldb * 2)};
     const cuuint32_t box[2] = {64, 64 * kKC};
-    rc = tiled_map(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT16, b, 2, dims, strides, box,
+    rc = tiled_map(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT16, o.b, 2, dims, strides, box,
                    CU_TENSOR_MAP_SWIZZLE_128B);
   }
-  if (rc) return rc;
-  rc = chunk_map(&tc, ep.c, M, N, ep.ldc);
-  if (!rc && ep.res != nullptr) rc = chunk_map(&tr, ep.res, M, N, ep.ldr);
+  if (!rc && !plain_out) rc = chunk_map(&tc, ep.c, M, N, ep.ldc);
+  if (!rc && !plain_out && ep.res != nullptr) rc = chunk_map(&tr, ep.res, M, N, ep.ldr);
   if (rc) return rc;
   const int64_t tiles = ceil_div(M, 256) * ceil_div(N, BN);
   if (tiles > INT32_MAX) return fail(TO_EUNSUPPORTED, "linear epilogue: too many tiles");
@@ -404,16 +410,11 @@ int launch_pair(const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
 
 }  // namespace
 
-// Runs the product on CTA pairs, or returns TO_EUNSUPPORTED (nothing launched, nothing recorded)
-// where the tiles do not apply: 16-bit output, rows of every operand 16-byte aligned, and enough
-// tiles to fill the SMs.
-int linear_pair_launch(int kind, const void* a, int64_t lda, const void* b,
-                       int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st) {
+// The tile width for a product, 0 where pairs do not pay (few tokens, or too few tiles to fill the
+// SMs without splitting K). Operands have to be of 16-byte aligned rows.
+int linear_pair_width(int kind, int64_t M, int64_t N) {
   const int e = kind == TO_F16 || kind == TO_BF16 ? 2 : 1;
-  if (M <= 128 || (ep.dtype != TO_F16 && ep.dtype != TO_BF16)) return TO_EUNSUPPORTED;
-  if (!aligned_rows(a, lda * e) || !aligned_rows(b, (e == 2 ? N : K) * e) ||
-      !aligned_rows(ep.c, ep.ldc * 2) || (ep.res && !aligned_rows(ep.res, ep.ldr * 2)))
-    return TO_EUNSUPPORTED;
+  if (M <= 128) return 0;
   const int64_t pairs = sm_count() / 2;
   // Tile width: the one whose rounds of tiles cost least; a tile's time is its width plus a fixed
   // part worth about 32 columns.
@@ -429,21 +430,31 @@ int linear_pair_launch(int kind, const void* a, int64_t lda, const void* b,
       best_cost = cost;
     }
   }
-  if (mt * ceil_div(N, best) * 2 < pairs) return TO_EUNSUPPORTED;  // split K instead
+  return mt * ceil_div(N, best) * 2 < pairs ? 0 : best;
+}
+
+// Runs the product on CTA pairs, or returns TO_EUNSUPPORTED (nothing launched, nothing recorded)
+// where the tiles do not apply.
+int linear_pair_launch(int kind, const LinOps& o, const LinEpi& ep, cudaStream_t st) {
+  const int e = kind == TO_F16 || kind == TO_BF16 ? 2 : 1;
+  const int best = linear_pair_width(kind, o.M, o.N);
+  if (best == 0 || !aligned_rows(o.a, o.lda * e) || !aligned_rows(o.b, o.ldb * e))
+    return TO_EUNSUPPORTED;
+  const bool plain = plain_output(ep);
   if (kind == TO_F16)
-    return best == 256 ? launch_pair<Kind::F16, 256>(a, lda, b, M, N, K, ep, st)
-                       : launch_pair<Kind::F16, 128>(a, lda, b, M, N, K, ep, st);
+    return best == 256 ? launch_pair<Kind::F16, 256>(o, plain, ep, st)
+                       : launch_pair<Kind::F16, 128>(o, plain, ep, st);
   if (kind == TO_BF16)
-    return best == 256 ? launch_pair<Kind::BF16, 256>(a, lda, b, M, N, K, ep, st)
-                       : launch_pair<Kind::BF16, 128>(a, lda, b, M, N, K, ep, st);
+    return best == 256 ? launch_pair<Kind::BF16, 256>(o, plain, ep, st)
+                       : launch_pair<Kind::BF16, 128>(o, plain, ep, st);
   auto run = [&](auto kd) {
     constexpr Kind KD = decltype(kd)::value;
     switch (best) {
-      case 256: return launch_pair<KD, 256>(a, lda, b, M, N, K, ep, st);
-      case 192: return launch_pair<KD, 192>(a, lda, b, M, N, K, ep, st);
-      case 160: return launch_pair<KD, 160>(a, lda, b, M, N, K, ep, st);
-      case 128: return launch_pair<KD, 128>(a, lda, b, M, N, K, ep, st);
-      default: return launch_pair<KD, 64>(a, lda, b, M, N, K, ep, st);
+      case 256: return launch_pair<KD, 256>(o, plain, ep, st);
+      case 192: return launch_pair<KD, 192>(o, plain, ep, st);
+      case 160: return launch_pair<KD, 160>(o, plain, ep, st);
+      case 128: return launch_pair<KD, 128>(o, plain, ep, st);
+      default: return launch_pair<KD, 64>(o, plain, ep, st);
     }
   };
   return kind == TO_I8 ? run(std::integral_constant<Kind, Kind::I8>{})

@@ -73,8 +73,7 @@ struct ChunkWriter {
   }
   // v: this lane's row of the chunk, scaled; bias: of its 32 columns, in shared memory. Straight
   // code per step, one uniform choice around each (see ActForm).
-  __device__ __forceinline__ void put(float* v, const float* bias, int col0, int row0, bool store) {
-    uint8_t* slab = slab0 + (cnt & 1) * kSlab;
+  __device__ __forceinline__ void finish_acts(float* v, const float* bias) {
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
       const float4 b = *reinterpret_cast<const float4*>(bias + i);
@@ -90,6 +89,41 @@ struct ChunkWriter {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = act_plain(v[i], form);
     }
+  }
+  // The chunk where the output or the residual is no TMA tensor (16-byte rows, 16-bit values): it
+  // turns in both slabs, so that a lane is a column and rows are read and written whole.
+  __device__ __forceinline__ void put_plain(float* v, const float* bias, int col0, int row0,
+                                            const LinEpi& ep, int M, int N, bool store) {
+    finish_acts(v, bias);
+    float* turn = reinterpret_cast<float*>(slab0);
+    __syncwarp();  // the previous chunk has been read
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      *reinterpret_cast<float4*>(turn + lane * 32 + ((c ^ (lane & 7)) << 2)) =
+          make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    __syncwarp();
+    const int n = col0 + lane, rows = min(32, M - row0);
+    if (n >= N || !store) return;
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += 8) {
+      float f[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int r = min(r0 + u, rows - 1);
+        f[u] = ep.res != nullptr ? ld_dtype(ep.res, (int64_t)(row0 + r) * ep.ldr + n, dtype) : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int r = r0 + u;
+        if (r >= rows) continue;
+        const float t = turn[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
+        st_dtype(ep.c, (int64_t)(row0 + r) * ep.ldc + n, dtype, t + f[u]);
+      }
+    }
+  }
+  __device__ __forceinline__ void put(float* v, const float* bias, int col0, int row0, bool store) {
+    finish_acts(v, bias);
+    uint8_t* slab = slab0 + (cnt & 1) * kSlab;
     // 16-byte pieces of 8 columns, swizzled as the TMA box is
     auto at = [&](int c) {
       return reinterpret_cast<uint4*>(slab + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4));
@@ -175,6 +209,12 @@ inline int chunk_map(CUtensorMap* out, const void* p, int64_t rows, int64_t cols
                    CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
+// Whether output or residual need the plain path: fp32, or rows that TMA cannot address.
+inline bool aligned_rows(const void* p, int64_t pitch);
+inline bool plain_output(const LinEpi& ep) {
+  return ep.dtype == TO_F32 || !aligned_rows(ep.c, ep.ldc * 2) ||
+         (ep.res != nullptr && !aligned_rows(ep.res, ep.ldr * 2));
+}
 inline bool aligned_rows(const void* p, int64_t pitch) {
   return ((reinterpret_cast<uint64_t>(p) | (uint64_t)pitch) & 15u) == 0;
 }

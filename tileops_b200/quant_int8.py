@@ -247,9 +247,14 @@ def _run_w8a8_bias_act(entry, op, a, b, a_s, b_s, block_n, block_k, m, n, k, bia
         b_s = b_s.to(torch.float32).contiguous()
     bias, residual, ldr, dst, ldc = _epilogue.prepare(shape, n, a, output_dtype, bias, residual,
                                                       out)
-    _lib.call(entry, a.data_ptr(), b.data_ptr(), a_s.data_ptr(), b_s.data_ptr(), _lib.ptr(bias),
-              code, _lib.ptr(residual), ldr, dst.data_ptr(), ldc,
-              _lib.DTYPE_CODES[output_dtype], m, n, k, block_n, block_k, _lib.stream_ptr(idx))
+    pa, pb = a.data_ptr(), b.data_ptr()
+    nbytes, ws, wp = 0, None, None
+    if m > 128 and (pa | pb | k) & 15:  # rows that need aligned copies
+        nbytes = _lib.load().to_w8a8_gemm_bias_act_workspace_size(pa, pb, m, n, k, block_k)
+        ws, wp = _epilogue.copies(nbytes, a)
+    _lib.call(entry, pa, pb, a_s.data_ptr(), b_s.data_ptr(), _lib.ptr(bias), code,
+              _lib.ptr(residual), ldr, dst.data_ptr(), ldc, _lib.DTYPE_CODES[output_dtype], m, n,
+              k, block_n, block_k, wp, nbytes, _lib.stream_ptr(idx))
     return _epilogue.finish(dst, out)
 
 
