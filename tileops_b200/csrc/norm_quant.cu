@@ -117,6 +117,14 @@ __device__ __forceinline__ Pack<uint8_t, V> codes_of(const Pack<float, V>& f, fl
   if constexpr (V == 1) {
     const float z = f.v[0] * c;
     o.v[0] = Q == kQE4M3 ? f32_to_e4m3(z) : (uint8_t)__float_as_uint(z + 12582912.0f);
+  } else if constexpr (V == 2) {
+    uint16_t w;
+    if constexpr (Q == kQE4M3)
+      w = f32x2_to_e4m3x2(f.v[0] * c, f.v[1] * c);
+    else
+      w = (uint16_t)__byte_perm(__float_as_uint(fmaf(f.v[0], c, 12582912.0f)),
+                                __float_as_uint(fmaf(f.v[1], c, 12582912.0f)), 0x0040);
+    *reinterpret_cast<uint16_t*>(o.v) = w;
   } else {
 #pragma unroll
     for (int k = 0; k < V / 4; ++k) {
@@ -144,15 +152,20 @@ __device__ __noinline__ uint8_t divided_code(float p, float rstd, float s) {
   return (uint8_t)rne_clamp_i8(z);
 }
 
-// Threads of a block at most: four packs a thread want 80 registers, fewer packs fit 64.
-template <int V, int MAXV> constexpr int kBlockMax = V > 1 && MAXV == 4 ? 384 : 1024;
+// Threads of a block at most, and blocks of an SM the registers are sized for. 32 values a thread
+// (four 16-byte packs of 16-bit values) want 80 registers, 16 or fewer fit 64. Many rows run on
+// blocks of 512 threads at most, so that an SM always holds two and one's loads cover the other's
+// arithmetic (a row of 13248 columns on one block of 832 threads per SM took three times as long);
+// what a longer row has left is re-read.
+template <int V, int MAXV> constexpr int kBlockMax = V * MAXV > 16 ? 384 : V * MAXV == 16 ? 512 : 1024;
+template <int V, int MAXV> constexpr int kBlocksMin = V * MAXV >= 16 ? 2 : 1;
 
 // One block per rows_per_block rows, a team of threads each. RES: with a residual and its output.
 // Loads are not guarded but clamped (rows and packs past the end re-read the last and count as
 // zero), so that all of a thread's loads go out together. 8192 x 8192 bf16 -> e4m3 with residual:
 // 87 us, 5.4 TB/s; a persistent form fed by bulk copies into shared memory ran no faster.
 template <typename T, int Q, int V, int MAXV, int MODE, bool RES>
-__global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlockMax<V, MAXV> == 384 ? 2 : 1)
+__global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlocksMin<V, MAXV>)
     k_norm_quant(const __grid_constant__ NormArgs a) {
   __shared__ float red[2][32];
   extern __shared__ unsigned gmax[];  // kGroupShared: [rows of the CTA][groups]
@@ -312,7 +325,7 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlockMax<V, MAXV> == 384 
     if (MAXV > 1 && shift >= 2) {
       // Lane i of a group works out the scale and the factor of the thread's i-th pack, once per
       // row instead of once per pack.
-      static_assert(MAXV <= 4 || V == 1, "lane i of a group of four or more");
+      static_assert(MAXV <= 4, "lane i of a group of four or more");
       float m[MAXV];
 #pragma unroll
       for (int i = 0; i < MAXV; ++i) m[i] = group_max(max_of(y[i], 0.f));
@@ -433,16 +446,27 @@ int launch_norm(NormArgs a, cudaStream_t st) {
   return check_launch("add_rms_norm_group_quant");
 }
 
+// Whether packs of v values can be used: the row length, the group, every row start.
+template <typename T>
+bool packs_of(const NormArgs& a, int v) {
+  const size_t b = v * sizeof(T);
+  return a.cols % v == 0 && a.G % v == 0 && aligned_to(a.x, b) && aligned_to(a.w, b) &&
+         a.ldx % v == 0 && aligned_to(a.q, v) &&
+         (!a.r || (aligned_to(a.r, b) && a.ldr % v == 0 && aligned_to(a.h, b) && a.ldh % v == 0));
+}
+
 template <typename T, int Q>
 int launch_norm_any(const NormArgs& a, cudaStream_t st) {
   constexpr int VV = 16 / sizeof(T);
-  const bool vec = a.cols % VV == 0 && a.G % VV == 0 && aligned16(a.x) && aligned16(a.w) &&
-                   a.ldx % VV == 0 && aligned_to(a.q, VV) &&
-                   (!a.r || (aligned16(a.r) && a.ldr % VV == 0)) &&
-                   (!a.h || (aligned16(a.h) && a.ldh % VV == 0));
-  if (!vec) {
-    if (a.G == a.cols) return launch_norm<T, Q, 1, 8, kGroupRow>(a, st);
-    return launch_norm<T, Q, 1, 8, kGroupShared>(a, st);
+  auto narrow = [&](auto v) {  // sixteen values a thread
+    constexpr int V = decltype(v)::value;
+    return a.G == a.cols ? launch_norm<T, Q, V, 16 / V, kGroupRow>(a, st)
+                         : launch_norm<T, Q, V, 16 / V, kGroupShared>(a, st);
+  };
+  if (!packs_of<T>(a, VV)) {
+    if (VV > 4 && packs_of<T>(a, 4)) return narrow(std::integral_constant<int, 4>{});
+    if (packs_of<T>(a, 2)) return narrow(std::integral_constant<int, 2>{});
+    return narrow(std::integral_constant<int, 1>{});
   }
   const int lanes = a.G / VV;
   const int mode = lanes <= 32 && (lanes & (lanes - 1)) == 0 ? kGroupLanes
@@ -450,9 +474,9 @@ int launch_norm_any(const NormArgs& a, cudaStream_t st) {
                                                             : kGroupShared;
   if (mode == kGroupShared) return launch_norm<T, Q, VV, 4, kGroupShared>(a, st);
   // Packs per thread: few rows (two per SM) take as few as keep a row in one block, for latency;
-  // many take four, for bytes in flight at few threads, or two where the row needs 1024 threads.
+  // many take four, for bytes in flight at few threads.
   const int64_t nvec = a.cols / VV;
-  const int maxv = a.rows <= 2 * sm_count() ? (nvec <= 1024 ? 1 : 2) : (nvec <= 4 * 384 ? 4 : 2);
+  const int maxv = a.rows > 2 * sm_count() || nvec > 2048 ? 4 : nvec <= 1024 ? 1 : 2;
   auto run = [&](auto m) {
     constexpr int MODE = decltype(m)::value;
     if (maxv == 1) return launch_norm<T, Q, VV, 1, MODE>(a, st);
