@@ -9,8 +9,9 @@
 //   tokens   [M, K], rows lda apart
 //
 // One token: bound by the weights' HBM stream. The K blocks of a column tile are split over the S
-// CTAs of a cluster so that every SM streams; the partial sums (int32 or fp32) are added through
-// distributed shared memory in rank order (deterministic, no workspace).
+// CTAs of a cluster so that every SM streams. Rank r finishes tokens r, r + S, ...: every rank stores
+// its partial sums (int32 or fp32) of a token into that rank's shared memory, one cluster barrier
+// later the owner adds them in rank order (deterministic, no workspace) and nobody reads a peer.
 //
 // Operands come by TMA when their rows are 16-byte aligned (PLAIN = false). Any other stride,
 // offset or size takes PLAIN: eight warps load the rows by aligned words, shift them together in
@@ -24,6 +25,9 @@
 #include <string.h>
 
 #include <algorithm>
+#include <array>
+#include <map>
+#include <mutex>
 #include <type_traits>
 
 #include "linear_epi.cuh"
@@ -50,14 +54,16 @@ struct NtCfg {
   static constexpr int kTpt = NT / (kEpiWarps / 4);  // tokens per epilogue thread
   static constexpr int kLoadWarps = PLAIN ? 8 : 0;
   static constexpr int kThreads = 128 + 32 * (kEpiWarps + kLoadWarps);
-  // Two CTAs per SM where registers allow: one CTA's prologue and reduction run under the other's
-  // stream. The loaders and the 64 running sums of a 128-token block-scaled tile do not fit twice.
-  static constexpr int kMinBlocks = (PLAIN || (BS && NT == 128)) ? 1 : 2;
-  static constexpr int kStages = (kMinBlocks == 2 ? 110 : 220) * 1024 / kStageBytes;
+  // Two CTAs per SM where they fit: one CTA's prologue and reduction run under the other's stream.
+  // The loaders' registers, and the sums of 128 tokens, do not fit twice.
+  static constexpr int kMinBlocks = (PLAIN || NT == 128) ? 1 : 2;
+  static constexpr int kSumBytes = (NT + 7) * 512;  // partial sums [token of this rank][rank][128]
+  static constexpr int kStages =
+      std::min(8, ((kMinBlocks == 2 ? 110 : 220) * 1024 - kSumBytes) / kStageBytes);
   static constexpr int kTmemCols = (BS ? 2 : 1) * NT < 32 ? 32 : (BS ? 2 : 1) * NT;
-  static constexpr size_t kSmem = (size_t)kStages * kStageBytes + 512;
+  static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kSumBytes + 512;
   static_assert((2 * kStages + 6) * 8 + 16 <= 512, "barrier area");
-  static_assert(128 * NT * 4 <= kStages * kStageBytes, "partial sums reuse the ring");
+  static_assert(kStages >= 3, "ring");
   static_assert(kSmem <= 232448, "shared memory");
 };
 
@@ -82,7 +88,8 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* sW = smem_raw;
   uint8_t* sX = smem_raw + (size_t)ST * C::kWBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw + (size_t)ST * C::kStageBytes);
+  uint8_t* sums = smem_raw + (size_t)ST * C::kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sums + C::kSumBytes);
   uint64_t* empty = full + ST;
   uint64_t* tfull = empty + ST;   // [2]; unscaled products use tfull[0]
   uint64_t* tempty = tfull + 2;   // [2]
@@ -126,6 +133,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
   const uint32_t tmem = *tmem_holder;
   bool ok = !misaligned;
   if (threadIdx.x == 0) grid_dependents_launch();  // the next kernel may set itself up
+  if (S > 1) cluster_arrive_relaxed();  // this CTA runs: its shared memory may be stored to
 
   if (!ok) {
     // nothing to do; fall through to the barriers and the teardown
@@ -281,14 +289,26 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
   const int n = n0 + q * 32 + lane;
   const bool n_ok = n < g.N;
   const LinEpi& ep = g.ep;
-  float* part = reinterpret_cast<float*>(smem_raw);  // [token][128] partial sums (ring reuse)
   float bias = 0.f, sb = 1.f;
+  // This thread's place in the sums, and the store of its partial sum of token tok = own * S + rank
+  // of the token's owner.
+  const uint32_t sum0 = smem_u32(sums + (q * 32 + lane) * 4);
+  auto give = [&](int own, int owner, uint32_t v) {
+    const uint32_t at = sum0 + (uint32_t)(own * S + rank) * 512u;
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(at, (uint32_t)owner)), "r"(v)
+                 : "memory");
+  };
+  int owner = epi ? half * C::kTpt % S : 0, own = epi ? half * C::kTpt / S : 0;
+  auto next_token = [&]() {
+    if (++owner == S) { owner = 0; ++own; }
+  };
   // One output of token tok: acc is its scaled sum.
   auto finish = [&](float acc, int tok, float res) {
     const float v = acc + bias;
     const float y = (ep.form.gated ? act_gated(v, ep.form) : act_plain(v, ep.form)) + res;
     st_dtype(ep.c, (int64_t)(t0 + tok) * ep.ldc + n, ep.dtype, y);
   };
+  if (S > 1) cluster_wait_acquire();  // so do the peers
   if (epi && ok) {
     grid_dependency_wait();
     if (n_ok && ep.bias != nullptr) bias = ld_dtype(ep.bias, n, ep.dtype);
@@ -326,11 +346,12 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
         __syncwarp();
         if (lane == 0) mbar_arrive(tempty + b);
       }
-      // The ring is idle: the last tfull covers every MMA that read it.
       if (ok) {
 #pragma unroll
-        for (int j = 0; j < C::kTpt; ++j)
-          part[(half * C::kTpt + j) * 128 + q * 32 + lane] = run[j];
+        for (int j = 0; j < C::kTpt; ++j) {
+          if (half * C::kTpt + j < tokens) give(own, owner, __float_as_uint(run[j]));
+          next_token();
+        }
       }
     } else {
       ok = mbar_wait_polled(tfull, 0, abort_flag, err);
@@ -343,66 +364,59 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
         tmem_ld16(lane_addr + (uint32_t)c, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          reinterpret_cast<uint32_t*>(part)[(tok0 + j) * 128 + q * 32 + lane] = r[j];
+        for (int j = 0; j < 16; ++j) {
+          if (tok0 + j < tokens) give(own, owner, r[j]);
+          next_token();
+        }
       }
     }
   }
-  // The sums go through shared memory, [token][128 columns], and a short loop over the tokens
-  // finishes them: this code runs once, so what it costs is the fetching of its instructions.
-  // Split K: rank r finishes tokens r, r + S, ..., each summed over the ranks in order. Otherwise
-  // every thread reads back its own tokens, so no barrier is needed.
-  if (S > 1) cluster_sync_all();
-  if (epi && ok && n_ok) {
-    // Tokens whose loads are in flight together (U) and partial sums per token (P).
-    auto tokens_loop = [&](auto u_tag, auto p_tag, int first, int last, int step) {
-      constexpr int U = decltype(u_tag)::value, P = decltype(p_tag)::value;
-      const uint32_t mine = smem_u32(part + q * 32 + lane);
+  // A short loop over this rank's tokens finishes them: this code runs once, so what it costs is the
+  // fetching of its instructions and the latency of its loads. Without a split every thread reads
+  // back what it stored, so no barrier is needed.
+  if (S > 1) cluster_arrive_release();
+  const int mine = (tokens - rank + S - 1) / S;  // tokens of this rank
+  const int i_step = S > 1 ? C::kEpiWarps / 4 : 1;
+  const int i_first = S > 1 ? half : half * C::kTpt;
+  const int i_last = S > 1 ? mine : min(mine, (half + 1) * C::kTpt);
+  constexpr int U = 4;  // tokens whose loads are in flight together
+  float res[U], sc[U];
+  auto operands = [&](int i0) {  // residual and scale of the next U tokens
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t t = t0 + rank + (int64_t)min(i0 + u * i_step, i_last - 1) * S;
+      res[u] = ep.res != nullptr ? ld_dtype(ep.res, t * ep.ldr + n, ep.dtype) : 0.f;
+      sc[u] = !BS && ep.a_s != nullptr ? __ldg(ep.a_s + t * ep.a_s_ld) * sb : 1.f;
+    }
+  };
+  const bool work = epi && ok && n_ok && i_first < i_last;
+  if (work) operands(i_first);
+  if (S > 1) cluster_wait_acquire();
+  if (work) {
 #pragma unroll 1
-      for (int tok = first; tok < last; tok += U * step) {
-        float res[U], sc[U];
-        uint32_t v[U][P];
+    for (int i0 = i_first; i0 < i_last; i0 += U * i_step) {
+      float acc[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int t = min(tok + u * step, last - 1);
-          if constexpr (P > 1) {
-#pragma unroll
-            for (int s = 0; s < P; ++s) {
-              v[u][s] = 0u;
-              if (s < S)
-                asm volatile("ld.shared::cluster.u32 %0, [%1];"
-                             : "=r"(v[u][s])
-                             : "r"(mapa_shared(mine + (uint32_t)t * 512u, (uint32_t)s))
-                             : "memory");
-            }
-          } else {
-            v[u][0] = reinterpret_cast<const uint32_t*>(part)[t * 128 + q * 32 + lane];
-          }
-          res[u] = ep.res != nullptr ? ld_dtype(ep.res, (int64_t)(t0 + t) * ep.ldr + n, ep.dtype)
-                                     : 0.f;
-          sc[u] = 1.f;
-          if (!BS && ep.a_s != nullptr)
-            sc[u] = __ldg(ep.a_s + (int64_t)(t0 + t) * ep.a_s_ld) * sb;
+      for (int u = 0; u < U; ++u) {
+        const int i = min(i0 + u * i_step, i_last - 1);
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(sums + (q * 32 + lane) * 4) +
+                             (size_t)i * S * 128;
+        uint32_t sum = at[0];
+        for (int s = 1; s < S; ++s) {
+          const uint32_t v = at[s * 128];
+          if (KD == Kind::I8 && !BS) sum += v;
+          else sum = __float_as_uint(__uint_as_float(sum) + __uint_as_float(v));
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          uint32_t sum = v[u][0];
-#pragma unroll
-          for (int s = 1; s < P; ++s) {
-            if (KD == Kind::I8 && !BS) sum += v[u][s];
-            else if (s < S) sum = __float_as_uint(__uint_as_float(sum) + __uint_as_float(v[u][s]));
-          }
-          const float acc = KD == Kind::I8 && !BS ? (float)(int32_t)sum : __uint_as_float(sum);
-          if (tok + u * step < last) finish(acc * sc[u], tok + u * step, res[u]);
-        }
+        acc[u] = (KD == Kind::I8 && !BS ? (float)(int32_t)sum : __uint_as_float(sum)) * sc[u];
       }
-    };
-    if (S > 1)
-      tokens_loop(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{},
-                  rank + half * S, tokens, S * (C::kEpiWarps / 4));
-    else
-      tokens_loop(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{},
-                  half * C::kTpt, min(tokens, (half + 1) * C::kTpt), 1);
+      float r_now[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) r_now[u] = res[u];
+      if (i0 + U * i_step < i_last) operands(i0 + U * i_step);  // in flight under the stores
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * i_step < i_last) finish(acc[u], rank + (i0 + u * i_step) * S, r_now[u]);
+    }
   }
   grid_dependency_wait();
   tc_fence_before();
@@ -411,7 +425,6 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
     tc_fence_after();
     tmem_dealloc<C::kTmemCols>(tmem);
   }
-  if (S > 1) cluster_sync_all();  // no rank leaves while a peer still reads its partial sums
 }
 
 // 2-D map of `rows` x `cols` elements, rows `pitch` bytes apart, boxes of 128 bytes x box_rows in
@@ -453,6 +466,40 @@ int strips_map(CUtensorMap* out, const void* p, int64_t K, int64_t N) {
   return TO_OK;
 }
 
+// Clusters of S blocks of `kern`, made for per_sm blocks of an SM, that the current device runs at
+// once (asked once per kernel and device; 0 if the driver cannot say).
+int clusters_at_once(const void* kern, int threads, size_t smem, int per_sm, int S) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, std::array<int, 9>> known;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  std::lock_guard<std::mutex> lock(mu);
+  std::array<int, 9>& n = known.try_emplace({kern, dev}, std::array<int, 9>{}).first->second;
+  if (n[0] == 0) {
+    for (int s = 1; s <= 8; ++s) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)(s * 1024), 1, 1);
+      cfg.blockDim = dim3((unsigned)threads, 1, 1);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)s;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int count = 0;
+      n[s] = cudaOccupancyMaxActiveClusters(&count, kern, &cfg) == cudaSuccess ? count : 0;
+    }
+    // The driver counts one block per SM; the kernels sized for two run two (their blocks were seen
+    // to start together, and the split that this count allows is the fastest).
+    const int times = n[1] <= sm_count() ? per_sm : 1;
+    for (int s = 1; s <= 8; ++s) n[s] *= times;
+    n[0] = 1;
+  }
+  return n[S];
+}
+
 int pow2_align(const void* p, int64_t pitch) {
   const uint64_t v = reinterpret_cast<uint64_t>(p) | (uint64_t)pitch | 16u;
   return (int)(v & (~v + 1));
@@ -467,11 +514,14 @@ int launch_nt(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, i
   if (ae != cudaSuccess) return cuda_fail(ae, "linear epilogue: shared memory attribute");
   const int64_t n_tiles = ceil_div(N, 128), m_tiles = ceil_div(M, NT);
   const int64_t kblocks = ceil_div(K, C::kBK);
-  // K split: as many CTAs as the SMs hold at once, at least two K blocks each, at most a
-  // portable cluster of eight.
-  const int64_t slots = (int64_t)sm_count() * C::kMinBlocks;
-  int64_t S = slots / (n_tiles * m_tiles);
-  S = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(S, 8), kblocks / 2));
+  // K split: the most CTAs that the SMs hold at once, at least two K blocks each, at most a portable
+  // cluster of eight. Clusters have to fit into the GPU's processor clusters whole, so the count
+  // comes from the driver. One token, 7168 x 7168 FP8 block-scaled, 56 tiles: two ways 21.6 us, three
+  // 16.3, four 14.1, and five, 280 CTAs for 296 places but two rounds, 20.0.
+  int64_t S = std::min<int64_t>(8, std::max<int64_t>(1, kblocks / 2));
+  while (S > 1 && n_tiles * m_tiles > clusters_at_once((const void*)kern, C::kThreads, C::kSmem,
+                                                       C::kMinBlocks, (int)S))
+    --S;
   if (n_tiles * S > INT32_MAX || m_tiles > 65535)
     return fail(TO_EUNSUPPORTED, "linear epilogue: too many tiles (M=%lld N=%lld)", (long long)M,
                 (long long)N);
@@ -519,9 +569,16 @@ int launch_nt(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, i
 template <Kind KD, bool BS, bool PLAIN>
 int launch_nt_tokens(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, int64_t K,
                      const LinEpi& ep, cudaStream_t st) {
-  if (M <= 16) return launch_nt<KD, 16, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
-  if (M <= 32) return launch_nt<KD, 32, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
-  if (M <= 64) return launch_nt<KD, 64, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
+  // The token tile: what covers the tokens in one column of tiles, or less where the blocks, K split
+  // as far as it goes, would leave SMs idle (each finishes its tokens one group after the other).
+  const int64_t n_tiles = ceil_div(N, 128);
+  const int64_t split = std::max<int64_t>(
+      1, std::min<int64_t>(8, ceil_div(K * KindTraits<KD>::kElemBytes, 128) / 2));
+  int nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  while (nt > 16 && n_tiles * ceil_div(M, nt) * split < sm_count()) nt /= 2;
+  if (nt == 16) return launch_nt<KD, 16, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
+  if (nt == 32) return launch_nt<KD, 32, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
+  if (nt == 64) return launch_nt<KD, 64, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
   return launch_nt<KD, 128, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
 }
 
