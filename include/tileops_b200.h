@@ -299,7 +299,8 @@ TO_API int to_gemm(const void* a, const void* b, void* c, int dtype, int64_t M, 
  * A [M,K] rows lda apart, B [K,N] dense, bias [N] or NULL, residual [M,N] rows ldr apart or NULL,
  * C [M,N] rows ldc apart, all of dtype F32, F16 or BF16; act one of TO_EPI_*. fp32 up to the one
  * rounding of C. C may be the residual; it must not overlap A or B. Any M, N, K (K = 0: the
- * epilogue of zeros). 16-bit operands run on tcgen05 tiles at any alignment, fp32 on SIMT tiles. */
+ * epilogue of zeros). 16-bit operands run on tcgen05 tiles at any alignment, fp32 on SIMT tiles.
+ * workspace as to_gemm_bias_act_workspace_size says. */
 #define TO_EPI_NONE 0
 #define TO_EPI_RELU 1
 #define TO_EPI_SILU 2
@@ -308,9 +309,8 @@ TO_API int to_gemm_bias_act(const void* a, int64_t lda, const void* b, const voi
                             const void* residual, int64_t ldr, void* c, int64_t ldc, int dtype,
                             int64_t M, int64_t N, int64_t K, void* workspace,
                             size_t workspace_bytes, void* stream);
-/* Scratch for padded copies of operands whose rows are not 16-byte aligned (0 for aligned ones and
- * for 128 tokens or fewer). It is optional: without it such a product runs on tiles that realign
- * the operands as they read them, several times slower at many tokens. */
+/* Bytes of scratch (16-byte aligned) for padded copies of the operands whose rows are not 16-byte
+ * aligned; 0 for aligned ones. */
 TO_API size_t to_gemm_bias_act_workspace_size(const void* a, int64_t lda, const void* b, int dtype,
                                               int64_t M, int64_t N, int64_t K);
 TO_API size_t to_w8a8_gemm_bias_act_workspace_size(const void* a, const void* b, int64_t M,

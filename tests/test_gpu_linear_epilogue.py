@@ -408,23 +408,29 @@ def test_w8a8_exact_many_tokens_ragged(cuda, codes, scales, dt, m, n, k):
     assert torch.equal(y, w8a8_exact(a, b, a_s, b_s, bn, bk, bias, "relu", res).to(dt))
 
 
-def test_without_workspace(cuda):
-    """The C entry without scratch for copies: the same product on tiles that realign as they read."""
-    m, n, k = 300, 1001, 333
-    gen = torch.Generator(device=cuda).manual_seed(5)
-    a = torch.randint(-3, 4, (m, k), generator=gen, device=cuda).half()
-    b = torch.randint(-2, 3, (k, n), generator=gen, device=cuda).half()
-    c = torch.empty(m, n, device=cuda, dtype=torch.float16)
-    lib = _lib.load()
-    f16 = _lib.DTYPE_CODES[torch.float16]
-    assert lib.to_gemm_bias_act_workspace_size(a.data_ptr(), k, b.data_ptr(), f16, m, n, k) > 0
-    assert lib.to_gemm_bias_act_workspace_size(a.data_ptr(), k, b.data_ptr(), f16, 128, n, k) == 0
-    for ws in (0, 1024):
-        buf = torch.empty(max(ws, 1), dtype=torch.uint8, device=cuda)
-        c.zero_()
-        _lib.call("to_gemm_bias_act", a.data_ptr(), k, b.data_ptr(), None, 0, None, n, c.data_ptr(),
-                  n, f16, m, n, k, buf.data_ptr() if ws else None, ws, _lib.stream_ptr())
-        assert torch.equal(c, exact_dense(a, b, None, None, None).half())
+def test_workspace_of_the_c_entries(cuda):
+    """Scratch for aligned copies: asked for exactly when a row is not 16-byte aligned, refused when
+    short, unaligned or missing, with nothing launched."""
+    m, n, k = 30, 1001, 333
+    a, b = torch.ones(m, k, device=cuda).half(), torch.ones(k, n, device=cuda).half()
+    c = torch.full((m, n), 7.0, device=cuda, dtype=torch.float16)
+    lib, f16 = _lib.load(), _lib.DTYPE_CODES[torch.float16]
+    need = lib.to_gemm_bias_act_workspace_size(a.data_ptr(), k, b.data_ptr(), f16, m, n, k)
+    assert need == m * 768 + k * 2048  # rows of 666 and 2002 bytes, padded to 128
+    assert lib.to_gemm_bias_act_workspace_size(1024, 336, 1024, f16, m, 1000, 333) == 0
+    assert lib.to_w8a8_gemm_bias_act_workspace_size(1024, 1024, m, n, 336, 336) == 0
+    assert lib.to_w8a8_gemm_bias_act_workspace_size(1024, 1024, m, n, k, k) == (m + n) * 384
+    buf = torch.empty(need + 16, dtype=torch.uint8, device=cuda)
+
+    def call(ws, size):
+        return lib.to_gemm_bias_act(a.data_ptr(), k, b.data_ptr(), None, 0, None, n, c.data_ptr(), n,
+                                    f16, m, n, k, ws, size, _lib.stream_ptr())
+
+    assert call(None, 0) == _lib.TO_ENOSPACE and call(buf.data_ptr(), need - 1) == _lib.TO_ENOSPACE
+    assert call(buf.data_ptr() + 8, need) == _lib.TO_EINVAL
+    assert bool((c == 7).all())
+    assert call(buf.data_ptr(), need) == _lib.TO_OK
+    assert bool((c == k).all())
 
 
 # Many tokens: several tiles per CTA pair, ragged last tiles, K of one slice, of an odd number of

@@ -91,7 +91,7 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
     bias, residual, ldr, dst, ldc = _epilogue.prepare((m, n), n, a, dtype, bias, residual, out)
     pa, pb, dc = a.data_ptr(), b.data_ptr(), _lib.DTYPE_CODES[dtype]
     nbytes, ws, wp = 0, None, None
-    if m > 128 and (pa | pb | 2 * lda | 2 * n) & 15:  # rows that need aligned copies
+    if (pa | pb | 2 * lda | 2 * n) & 15 and dtype is not torch.float32:  # aligned copies
         nbytes = _lib.load().to_gemm_bias_act_workspace_size(pa, lda, pb, dc, m, n, k)
         ws, wp = _epilogue.copies(nbytes, a)
     _lib.call("to_gemm_bias_act", pa, lda, pb, _lib.ptr(bias), code, _lib.ptr(residual), ldr,

@@ -414,7 +414,7 @@ int launch_bs(const LinOps& o, bool plain_out, const LinEpi& ep, cudaStream_t st
 
 // The tile width for a block-scaled product, 0 where these tiles do not pay or apply: column blocks
 // have to be whole 32-column chunks, and the tiles to fill the SMs.
-int linear_bs_width(int64_t M, int64_t N, int64_t bn) {
+static int bs_width(int64_t M, int64_t N, int64_t bn) {
   if (M <= 64 || (bn % 32 != 0 && bn < N)) return 0;
   // The width whose rounds of tiles cost least; a tile's time is its width plus a fixed part worth
   // about 32 columns.
@@ -436,7 +436,7 @@ int linear_bs_width(int64_t M, int64_t N, int64_t bn) {
 // Runs it, or returns TO_EUNSUPPORTED (nothing launched, nothing recorded). Rows of A and B have to
 // be 16-byte aligned.
 int linear_bs_launch(int kind, const LinOps& o, const LinEpi& ep, cudaStream_t st) {
-  const int best = linear_bs_width(o.M, o.N, ep.bn);
+  const int best = bs_width(o.M, o.N, ep.bn);
   if (best == 0 || !aligned_rows(o.a, o.lda) || !aligned_rows(o.b, o.ldb)) return TO_EUNSUPPORTED;
   const bool plain = plain_output(ep);
   auto run = [&](auto kd) {

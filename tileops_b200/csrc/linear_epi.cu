@@ -4,13 +4,11 @@
 
 namespace tob {
 namespace sm100 {
-int linear_nt_launch(int kind, bool block_scaled, const void* x, int64_t ldx, const void* w,
-                     int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st);
+int linear_nt_launch(int kind, bool block_scaled, const LinOps& o, const LinEpi& ep,
+                     cudaStream_t st);
 // TO_EUNSUPPORTED (nothing launched) where the tiles do not apply.
 int linear_pair_launch(int kind, const LinOps& o, const LinEpi& ep, cudaStream_t st);
-int linear_pair_width(int kind, int64_t M, int64_t N);
 int linear_bs_launch(int kind, const LinOps& o, const LinEpi& ep, cudaStream_t st);
-int linear_bs_width(int64_t M, int64_t N, int64_t bn);
 }
 int64_t linear_relay_bytes(int kind, const LinOps& o);
 int linear_relay(int kind, LinOps* o, void* ws, cudaStream_t st);
@@ -21,30 +19,21 @@ int linear_w8a8_simt_launch(bool fp8, const void* a, const void* b, int64_t M, i
 
 namespace {
 
-// Tokens from which a product is worth aligned copies of operands that TMA cannot read: below, one
-// column of tiles reads the weights once at any alignment; above, every further 128 tokens would
-// realign them again.
-constexpr int64_t kRelayTokens = 128;
-
 LinOps make_ops(const void* a, int64_t lda, const void* b, int64_t M, int64_t N, int64_t K,
                 bool b_mn) {
   return LinOps{a, b, lda, b_mn ? N : K, K, b_mn ? N : K, M, N, K};
 }
 
-int64_t relay_bytes(int kind, const LinOps& o) {
-  return o.M > kRelayTokens ? linear_relay_bytes(kind, o) : 0;
-}
-
-// Many tokens: CTA-pair tiles, or folding tiles with block scales, over aligned copies where need be
-// and the caller's workspace allows; few tokens, a small grid, or no workspace: weights as rows.
-int tensor_core_launch(int kind, bool block_scaled, LinOps o, LinEpi ep, void* ws, size_t ws_bytes,
-                       cudaStream_t st) {
-  const LinOps given = o;
-  const bool tiles = (block_scaled ? sm100::linear_bs_width(o.M, o.N, ep.bn)
-                                   : sm100::linear_pair_width(kind, o.M, o.N)) != 0;
-  const int64_t need = tiles ? relay_bytes(kind, o) : 0;
-  if (need > 0 && ws != nullptr && (int64_t)ws_bytes >= need &&
-      (reinterpret_cast<uint64_t>(ws) & 15u) == 0) {
+// Many tokens: CTA-pair tiles, or folding tiles with block scales; few tokens or a small grid: weights
+// as rows. All of them over aligned copies of the operands that TMA cannot read.
+int tensor_core_launch(const char* op, int kind, bool block_scaled, LinOps o, LinEpi ep, void* ws,
+                       size_t ws_bytes, cudaStream_t st) {
+  const int64_t need = linear_relay_bytes(kind, o);
+  if (need > 0) {
+    if (!ws || (int64_t)ws_bytes < need)
+      return fail(TO_ENOSPACE, "%s: workspace of %zu bytes is too small (%lld)", op, ws_bytes,
+                  (long long)need);
+    if (!aligned16(ws)) return fail(TO_EINVAL, "%s: workspace is not 16-byte aligned", op);
     const int rc = linear_relay(kind, &o, ws, st);
     if (rc) return rc;
     ep.early_weights = 0;  // the copies are the previous kernel's output
@@ -52,8 +41,7 @@ int tensor_core_launch(int kind, bool block_scaled, LinOps o, LinEpi ep, void* w
   const int rc = block_scaled ? sm100::linear_bs_launch(kind, o, ep, st)
                               : sm100::linear_pair_launch(kind, o, ep, st);
   if (rc != TO_EUNSUPPORTED) return rc;
-  return sm100::linear_nt_launch(kind, block_scaled, given.a, given.lda, given.b, given.M, given.N,
-                                 given.K, ep, st);
+  return sm100::linear_nt_launch(kind, block_scaled, o, ep, st);
 }
 
 // Fills the epilogue common to both products; TO_OK or a recorded failure.
@@ -104,7 +92,7 @@ int w8a8_epi_entry(bool fp8, const void* a, const void* b, const float* a_s, con
   if (kt > 1 && bk % 128 != 0)
     return linear_w8a8_simt_launch(fp8, a, b, M, N, K, ep.bn, bk, ep, st);
   ep.kb_per_scale = kt > 1 ? (int)(bk / 128) : 1;
-  return tensor_core_launch(fp8 ? TO_E4M3 : TO_I8, kt > 1, make_ops(a, K, b, M, N, K, false), ep,
+  return tensor_core_launch(op, fp8 ? TO_E4M3 : TO_I8, kt > 1, make_ops(a, K, b, M, N, K, false), ep,
                             ws, ws_bytes, st);
 }
 
@@ -116,13 +104,13 @@ extern "C" {
 size_t to_gemm_bias_act_workspace_size(const void* a, int64_t lda, const void* b, int dtype,
                                        int64_t M, int64_t N, int64_t K) {
   if ((dtype != TO_F16 && dtype != TO_BF16) || M <= 0 || N <= 0 || K <= 0) return 0;
-  return (size_t)tob::relay_bytes(dtype, tob::make_ops(a, lda, b, M, N, K, true));
+  return (size_t)tob::linear_relay_bytes(dtype, tob::make_ops(a, lda, b, M, N, K, true));
 }
 
 size_t to_w8a8_gemm_bias_act_workspace_size(const void* a, const void* b, int64_t M, int64_t N,
                                             int64_t K, int64_t block_k) {
   if (M <= 0 || N <= 0 || K <= 0 || block_k <= 0 || (block_k < K && block_k % 128 != 0)) return 0;
-  return (size_t)tob::relay_bytes(TO_I8, tob::make_ops(a, K, b, M, N, K, false));
+  return (size_t)tob::linear_relay_bytes(TO_I8, tob::make_ops(a, K, b, M, N, K, false));
 }
 
 int to_gemm_bias_act(const void* a, int64_t lda, const void* b, const void* bias, int act,
@@ -144,7 +132,7 @@ int to_gemm_bias_act(const void* a, int64_t lda, const void* b, const void* bias
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == TO_F32 || K == 0)
     return linear_dense_simt_launch(a, lda, b, M, N, K, ep, st);
-  return tensor_core_launch(dtype, false, make_ops(a, lda, b, M, N, K, true), ep, workspace,
+  return tensor_core_launch(op, dtype, false, make_ops(a, lda, b, M, N, K, true), ep, workspace,
                             workspace_bytes, st);
 }
 

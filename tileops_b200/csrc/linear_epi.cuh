@@ -87,6 +87,16 @@ __device__ __forceinline__ float ld_dtype(const void* p, int64_t i, int dtype) {
   if (dtype == TO_F16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
   return reinterpret_cast<const float*>(p)[i];
 }
+// The same in two steps, load and conversion, without a branch between loads: a choice of type
+// around each load makes the next one wait for it.
+__device__ __forceinline__ uint32_t ld_raw(const void* p, int64_t i, bool wide) {
+  return wide ? reinterpret_cast<const uint32_t*>(p)[i]
+              : (uint32_t)reinterpret_cast<const uint16_t*>(p)[i];
+}
+__device__ __forceinline__ float raw_to_f32(uint32_t v, int dtype) {
+  const float h = __half2float(__ushort_as_half((unsigned short)v));
+  return dtype == TO_F16 ? h : __uint_as_float(dtype == TO_BF16 ? v << 16 : v);
+}
 __device__ __forceinline__ void st_dtype(void* p, int64_t i, int dtype, float v) {
   if (dtype == TO_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
   else if (dtype == TO_F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);

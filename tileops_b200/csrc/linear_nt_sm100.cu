@@ -13,12 +13,10 @@
 // its partial sums (int32 or fp32) of a token into that rank's shared memory, one cluster barrier
 // later the owner adds them in rank order (deterministic, no workspace) and nobody reads a peer.
 //
-// Operands come by TMA when their rows are 16-byte aligned (PLAIN = false). Any other stride,
-// offset or size takes PLAIN: eight warps load the rows by aligned words, shift them together in
-// registers and store them in the same swizzled layout.
+// Operands come by TMA: their rows are 16-byte aligned, by themselves or as padded copies.
 //
 // Roles: warp 0 weight copies, warp 1 MMA issue and TMEM, warp 2 token copies, warp 3 idle, then
-// kEpiWarps epilogue warps (lane quarter = warp % 4) and, with PLAIN, kLoadWarps loaders.
+// kEpiWarps epilogue warps (lane quarter = warp % 4).
 // Every wait is bounded (kWaitLimitNs); on expiry all roles unwind through the same barriers.
 #include <cudaTypedefs.h>
 
@@ -31,7 +29,6 @@
 #include <type_traits>
 
 #include "linear_epi.cuh"
-#include "realign.cuh"
 #include "sm100.cuh"
 
 namespace tob {
@@ -41,7 +38,7 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode();
 
 namespace {
 
-template <Kind KD, int NT, bool BS, bool PLAIN>
+template <Kind KD, int NT, bool BS>
 struct NtCfg {
   static_assert(NT == 16 || NT == 32 || NT == 64 || NT == 128, "token tile");
   static constexpr int kElem = KindTraits<KD>::kElemBytes;
@@ -52,11 +49,10 @@ struct NtCfg {
   static constexpr int kStageBytes = kWBytes + kXBytes;
   static constexpr int kEpiWarps = NT >= 64 ? 8 : 4;
   static constexpr int kTpt = NT / (kEpiWarps / 4);  // tokens per epilogue thread
-  static constexpr int kLoadWarps = PLAIN ? 8 : 0;
-  static constexpr int kThreads = 128 + 32 * (kEpiWarps + kLoadWarps);
+  static constexpr int kThreads = 128 + 32 * kEpiWarps;
   // Two CTAs per SM where they fit: one CTA's prologue and reduction run under the other's stream.
-  // The loaders' registers, and the sums of 128 tokens, do not fit twice.
-  static constexpr int kMinBlocks = (PLAIN || NT == 128) ? 1 : 2;
+  // The sums of 128 tokens do not fit twice.
+  static constexpr int kMinBlocks = NT == 128 ? 1 : 2;
   static constexpr int kSumBytes = (NT + 7) * 512;  // partial sums [token of this rank][rank][128]
   static constexpr int kStages =
       std::min(8, ((kMinBlocks == 2 ? 110 : 220) * 1024 - kSumBytes) / kStageBytes);
@@ -70,19 +66,15 @@ struct NtCfg {
 struct NtArgs {
   int M, N, K, splits;
   int strips3d;       // MN-major weights through the 3-D strip map (N % 64 == 0)
-  // PLAIN operands
-  const uint8_t* w;
-  const uint8_t* x;
-  int64_t w_pitch, x_pitch;  // bytes between rows
   LinEpi ep;
 };
 
-template <Kind KD, int NT, bool BS, bool PLAIN>
-__global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
-                                  NtCfg<KD, NT, BS, PLAIN>::kMinBlocks)
+template <Kind KD, int NT, bool BS>
+__global__ void __launch_bounds__(NtCfg<KD, NT, BS>::kThreads,
+                                  NtCfg<KD, NT, BS>::kMinBlocks)
     k_linear_nt(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                 const __grid_constant__ NtArgs g, int* err) {
-  using C = NtCfg<KD, NT, BS, PLAIN>;
+  using C = NtCfg<KD, NT, BS>;
   using Tr = KindTraits<KD>;
   constexpr int ST = C::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -110,7 +102,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
-      mbar_init(full + s, PLAIN ? C::kLoadWarps : 2);
+      mbar_init(full + s, 2);
       mbar_init(empty + s, 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -120,10 +112,8 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    if (!PLAIN) {
-      prefetch_tmap(&tmW);
-      prefetch_tmap(&tmX);
-    }
+    prefetch_tmap(&tmW);
+    prefetch_tmap(&tmX);
     if (misaligned && err) atomicExch(err, (int)kErrSmemAlign);
   }
   if (warp == 1) tmem_alloc<C::kTmemCols>(tmem_holder);
@@ -137,7 +127,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
 
   if (!ok) {
     // nothing to do; fall through to the barriers and the teardown
-  } else if (!PLAIN && (warp == 0 || warp == 2)) {
+  } else if (warp == 0 || warp == 2) {
     // ------------------------------------------------------------ TMA: weights / tokens
     if (lane == 0) {
       const bool wts = warp == 0;
@@ -213,77 +203,10 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
         }
       }
     }
-  } else if (PLAIN && warp >= 4 + C::kEpiWarps) {
-    // ------------------------------------------------------------ loaders (any alignment)
-    if constexpr (PLAIN) {
-      // A warp takes groups of four 128-byte rows, a lane one 16-byte chunk of a row.
-      constexpr int kGroups = (128 + NT) / 4;
-      constexpr int kMine = (kGroups + C::kLoadWarps - 1) / C::kLoadWarps;
-      const int lw = warp - 4 - C::kEpiWarps;
-      const int chunk = lane & 7;
-      const int64_t row_bytes = (int64_t)g.K * C::kElem;
-      const int64_t w_rows = C::kMn ? g.K : g.N;
-      const int64_t w_bytes = C::kMn ? (int64_t)g.N * 2 : row_bytes;
-      const uint8_t* w_hi = g.w + (w_rows - 1) * g.w_pitch + w_bytes;
-      const uint8_t* x_hi = g.x + (int64_t)(g.M - 1) * g.x_pitch + row_bytes;
-      grid_dependency_wait();
-      constexpr int kBatch = 4;  // 16-byte pieces whose loads a lane has in flight
-      for (int it = 0; it < kb_n; ++it) {
-        const int s = it % ST;
-        const int64_t kbyte = (int64_t)(kb_lo + it) * 128;
-        bool waited = it < ST;
-#pragma unroll
-        for (int i0 = 0; i0 < kMine; i0 += kBatch) {
-          Unaligned16 v[kBatch];
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const int row = (lw + (i0 + i) * C::kLoadWarps) * 4 + (lane >> 3);
-            if (row < 128) {
-              int64_t r, off;  // source row and byte offset in it
-              if (C::kMn) {
-                r = (int64_t)(kb_lo + it) * 64 + (row & 63);
-                off = (int64_t)(n0 + (row & 64)) * 2 + chunk * 16;
-              } else {
-                r = n0 + row;
-                off = kbyte + chunk * 16;
-              }
-              const int64_t left = r < w_rows ? w_bytes - off : 0;
-              v[i].issue(g.w + r * g.w_pitch + off, (int)max((int64_t)0, min((int64_t)16, left)),
-                         g.w, w_hi);
-            } else {
-              const int t = row - 128;
-              const int64_t off = kbyte + chunk * 16;
-              const int64_t left = t < tokens ? row_bytes - off : 0;
-              v[i].issue(g.x + (int64_t)(t0 + t) * g.x_pitch + off,
-                         (int)max((int64_t)0, min((int64_t)16, left)), g.x, x_hi);
-            }
-          }
-          if (!waited) {
-            if (!mbar_wait_polled(empty + s, ((uint32_t)(it / ST) & 1u) ^ 1, abort_flag, err)) {
-              ok = false;
-              break;
-            }
-            waited = true;
-          }
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const int row = (lw + (i0 + i) * C::kLoadWarps) * 4 + (lane >> 3);
-            if (row >= 128 + NT) continue;
-            uint8_t* tile = row < 128 ? sW + (size_t)s * C::kWBytes : sX + (size_t)s * C::kXBytes;
-            const int r = row < 128 ? row : row - 128;
-            *reinterpret_cast<uint4*>(tile + r * 128 + ((chunk ^ (r & 7)) << 4)) = v[i].finish();
-          }
-        }
-        if (!ok) break;
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full + s);
-      }
-    }
   }
 
   // -------------------------------------------------------------- epilogue
-  const bool epi = warp >= 4 && warp < 4 + C::kEpiWarps;
+  const bool epi = warp >= 4;
   const int q = warp & 3;                     // TMEM lane quarter
   const int half = (warp - 4) >> 2;           // which kTpt tokens of the tile
   const int n = n0 + q * 32 + lane;
@@ -380,12 +303,13 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
   const int i_first = S > 1 ? half : half * C::kTpt;
   const int i_last = S > 1 ? mine : min(mine, (half + 1) * C::kTpt);
   constexpr int U = 4;  // tokens whose loads are in flight together
-  float res[U], sc[U];
+  uint32_t res[U];
+  float sc[U];
   auto operands = [&](int i0) {  // residual and scale of the next U tokens
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t t = t0 + rank + (int64_t)min(i0 + u * i_step, i_last - 1) * S;
-      res[u] = ep.res != nullptr ? ld_dtype(ep.res, t * ep.ldr + n, ep.dtype) : 0.f;
+      res[u] = ep.res == nullptr ? 0u : ld_raw(ep.res, t * ep.ldr + n, ep.dtype == TO_F32);
       sc[u] = !BS && ep.a_s != nullptr ? __ldg(ep.a_s + t * ep.a_s_ld) * sb : 1.f;
     }
   };
@@ -411,7 +335,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS, PLAIN>::kThreads,
       }
       float r_now[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) r_now[u] = res[u];
+      for (int u = 0; u < U; ++u) r_now[u] = raw_to_f32(res[u], ep.dtype);
       if (i0 + U * i_step < i_last) operands(i0 + U * i_step);  // in flight under the stores
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -449,11 +373,11 @@ int rows_map(CUtensorMap* out, const void* p, int64_t rows, int64_t cols, int64_
 }
 
 // Weights [K, N], N % 64 == 0, as {64 columns, K rows, N / 64 strips}: one box of two strips.
-int strips_map(CUtensorMap* out, const void* p, int64_t K, int64_t N) {
+int strips_map(CUtensorMap* out, const void* p, int64_t K, int64_t N, int64_t pitch) {
   auto encode = get_encode();
   if (!encode) return fail(TO_ECUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
   cuuint64_t dims[3] = {64, (cuuint64_t)K, (cuuint64_t)(N / 64)};
-  cuuint64_t strides[2] = {(cuuint64_t)(N * 2), 128};
+  cuuint64_t strides[2] = {(cuuint64_t)pitch, 128};
   cuuint32_t box[3] = {64, 64, 2};
   cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(p), dims,
@@ -500,18 +424,13 @@ int clusters_at_once(const void* kern, int threads, size_t smem, int per_sm, int
   return n[S];
 }
 
-int pow2_align(const void* p, int64_t pitch) {
-  const uint64_t v = reinterpret_cast<uint64_t>(p) | (uint64_t)pitch | 16u;
-  return (int)(v & (~v + 1));
-}
-
-template <Kind KD, int NT, bool BS, bool PLAIN>
-int launch_nt(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, int64_t K,
-              const LinEpi& ep, cudaStream_t st) {
-  using C = NtCfg<KD, NT, BS, PLAIN>;
-  auto kern = k_linear_nt<KD, NT, BS, PLAIN>;
+template <Kind KD, int NT, bool BS>
+int launch_nt(const LinOps& o, const LinEpi& ep, cudaStream_t st) {
+  using C = NtCfg<KD, NT, BS>;
+  auto kern = k_linear_nt<KD, NT, BS>;
   const cudaError_t ae = ensure_smem_attr((const void*)kern, (int)C::kSmem);
   if (ae != cudaSuccess) return cuda_fail(ae, "linear epilogue: shared memory attribute");
+  const int64_t M = o.M, N = o.N, K = o.K;
   const int64_t n_tiles = ceil_div(N, 128), m_tiles = ceil_div(M, NT);
   const int64_t kblocks = ceil_div(K, C::kBK);
   // K split: the most CTAs that the SMs hold at once, at least two K blocks each, at most a portable
@@ -531,22 +450,15 @@ int launch_nt(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, i
   g.N = (int)N;
   g.K = (int)K;
   g.splits = (int)S;
-  g.strips3d = C::kMn && N % 64 == 0;
-  g.w = (const uint8_t*)w;
-  g.x = (const uint8_t*)x;
-  g.w_pitch = (C::kMn ? N : K) * C::kElem;
-  g.x_pitch = ldx * C::kElem;
+  g.strips3d = C::kMn && o.b_in % 64 == 0;
   g.ep = ep;
   CUtensorMap tw, tx;
-  memset(&tw, 0, sizeof(tw));
-  memset(&tx, 0, sizeof(tx));
-  if (!PLAIN) {
-    int rc = !C::kMn      ? rows_map(&tw, w, N, K, g.w_pitch, C::kElem, 128)
-             : g.strips3d ? strips_map(&tw, w, K, N)
-                          : rows_map(&tw, w, K, N, g.w_pitch, C::kElem, 64);
-    if (!rc) rc = rows_map(&tx, x, M, K, g.x_pitch, C::kElem, NT);
-    if (rc) return rc;
-  }
+  const int64_t w_pitch = o.ldb * C::kElem;
+  int rc = !C::kMn      ? rows_map(&tw, o.b, N, o.b_in, w_pitch, C::kElem, 128)
+           : g.strips3d ? strips_map(&tw, o.b, K, o.b_in, w_pitch)
+                        : rows_map(&tw, o.b, K, o.b_in, w_pitch, C::kElem, 64);
+  if (!rc) rc = rows_map(&tx, o.a, M, o.a_k, o.lda * C::kElem, C::kElem, NT);
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(n_tiles * S), (unsigned)m_tiles, 1);
   cfg.blockDim = dim3(C::kThreads, 1, 1);
@@ -566,9 +478,9 @@ int launch_nt(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, i
   return check_launch("linear epilogue");
 }
 
-template <Kind KD, bool BS, bool PLAIN>
-int launch_nt_tokens(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, int64_t K,
-                     const LinEpi& ep, cudaStream_t st) {
+template <Kind KD, bool BS>
+int launch_nt_any(const LinOps& o, const LinEpi& ep, cudaStream_t st) {
+  const int64_t M = o.M, N = o.N, K = o.K;
   // The token tile: what covers the tokens in one column of tiles, or less where the blocks, K split
   // as far as it goes, would leave SMs idle (each finishes its tokens one group after the other).
   const int64_t n_tiles = ceil_div(N, 128);
@@ -576,37 +488,27 @@ int launch_nt_tokens(const void* x, int64_t ldx, const void* w, int64_t M, int64
       1, std::min<int64_t>(8, ceil_div(K * KindTraits<KD>::kElemBytes, 128) / 2));
   int nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   while (nt > 16 && n_tiles * ceil_div(M, nt) * split < sm_count()) nt /= 2;
-  if (nt == 16) return launch_nt<KD, 16, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
-  if (nt == 32) return launch_nt<KD, 32, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
-  if (nt == 64) return launch_nt<KD, 64, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
-  return launch_nt<KD, 128, BS, PLAIN>(x, ldx, w, M, N, K, ep, st);
-}
-
-template <Kind KD, bool BS>
-int launch_nt_any(const void* x, int64_t ldx, const void* w, int64_t M, int64_t N, int64_t K,
-                  const LinEpi& ep, cudaStream_t st) {
-  constexpr int e = KindTraits<KD>::kElemBytes;
-  const int64_t w_pitch = (e == 2 ? N : K) * e;
-  const bool tma = pow2_align(w, w_pitch) == 16 && pow2_align(x, ldx * e) == 16;
-  return tma ? launch_nt_tokens<KD, BS, false>(x, ldx, w, M, N, K, ep, st)
-             : launch_nt_tokens<KD, BS, true>(x, ldx, w, M, N, K, ep, st);
+  if (nt == 16) return launch_nt<KD, 16, BS>(o, ep, st);
+  if (nt == 32) return launch_nt<KD, 32, BS>(o, ep, st);
+  if (nt == 64) return launch_nt<KD, 64, BS>(o, ep, st);
+  return launch_nt<KD, 128, BS>(o, ep, st);
 }
 
 }  // namespace
 
 // Entry of this file: `kind` one of TO_I8, TO_E4M3 (weights [N, K]), TO_F16, TO_BF16 (weights
 // [K, N]); block_scaled: ep's scales change every ep.kb_per_scale 128-byte K slices.
-int linear_nt_launch(int kind, bool block_scaled, const void* x, int64_t ldx, const void* w,
-                     int64_t M, int64_t N, int64_t K, const LinEpi& ep, cudaStream_t st) {
+int linear_nt_launch(int kind, bool block_scaled, const LinOps& o, const LinEpi& ep,
+                     cudaStream_t st) {
   switch (kind) {
-    case TO_F16: return launch_nt_any<Kind::F16, false>(x, ldx, w, M, N, K, ep, st);
-    case TO_BF16: return launch_nt_any<Kind::BF16, false>(x, ldx, w, M, N, K, ep, st);
+    case TO_F16: return launch_nt_any<Kind::F16, false>(o, ep, st);
+    case TO_BF16: return launch_nt_any<Kind::BF16, false>(o, ep, st);
     case TO_I8:
-      return block_scaled ? launch_nt_any<Kind::I8, true>(x, ldx, w, M, N, K, ep, st)
-                          : launch_nt_any<Kind::I8, false>(x, ldx, w, M, N, K, ep, st);
+      return block_scaled ? launch_nt_any<Kind::I8, true>(o, ep, st)
+                          : launch_nt_any<Kind::I8, false>(o, ep, st);
     case TO_E4M3:
-      return block_scaled ? launch_nt_any<Kind::E4M3, true>(x, ldx, w, M, N, K, ep, st)
-                          : launch_nt_any<Kind::E4M3, false>(x, ldx, w, M, N, K, ep, st);
+      return block_scaled ? launch_nt_any<Kind::E4M3, true>(o, ep, st)
+                          : launch_nt_any<Kind::E4M3, false>(o, ep, st);
   }
   return fail(TO_EUNSUPPORTED, "linear epilogue: operand dtype %s", dtype_name(kind));
 }

@@ -263,6 +263,19 @@ __global__ void __launch_bounds__(kThreadsP, 1)
     int fill = 0;  // accumulator fills read
     bool ok = true;
     auto chunk_col = [&](int j) { return (2 * j + eg) * 32; };  // this warp's j-th chunk
+    // Scale and bias of this thread's column of a tile, read one tile ahead.
+    static_assert(BN <= 32 * kEpiWarpsT, "a thread per column");
+    const int col = (int)threadIdx.x - 64;
+    float scale_next = 1.f, bias_next = 0.f;
+    auto read_cols = [&](int t) {
+      if (t >= tiles || col >= BN) return;
+      int mt, nt;
+      band_tile(t, m_tiles, n_tiles, g.band, mt, nt);
+      const int n = min(nt * BN + col, g.N - 1);
+      if (ep.b_s != nullptr) scale_next = __ldg(ep.b_s + (int64_t)(n / ep.bn) * ep.b_s_ld);
+      if (ep.bias != nullptr) bias_next = ld_dtype(ep.bias, n, ep.dtype);
+    };
+    read_cols(pair);
     for (int t = pair; t < tiles; t += pairs) {
       int mt, nt;
       band_tile(t, m_tiles, n_tiles, g.band, mt, nt);
@@ -276,12 +289,12 @@ __global__ void __launch_bounds__(kThreadsP, 1)
       if (!rows_in) mine = 0;
       // Scale and bias of the tile's columns.
       epi_barrier();  // every warp is done with the previous tile's
-      for (int i = threadIdx.x - 64; i < BN; i += kEpiWarpsT * 32) {
-        const int n = min(n0 + i, g.N - 1);
-        scale[i] = ep.b_s != nullptr ? __ldg(ep.b_s + (int64_t)(n / ep.bn) * ep.b_s_ld) : 1.f;
-        bias[i] = ep.bias != nullptr ? ld_dtype(ep.bias, n, ep.dtype) : 0.f;
+      if (col < BN) {
+        scale[col] = scale_next;
+        bias[col] = bias_next;
       }
       epi_barrier();
+      read_cols(t + pairs);
       // After a failed wait a warp still walks the tiles: the others count on it at the barriers.
       if (!ok) continue;
       if (mine > 0) wr.fetch(0, n0 + chunk_col(0), row0);
@@ -412,7 +425,7 @@ int launch_pair(const LinOps& o, bool plain_out, const LinEpi& ep, cudaStream_t 
 
 // The tile width for a product, 0 where pairs do not pay (few tokens, or too few tiles to fill the
 // SMs without splitting K). Operands have to be of 16-byte aligned rows.
-int linear_pair_width(int kind, int64_t M, int64_t N) {
+static int pair_width(int kind, int64_t M, int64_t N) {
   const int e = kind == TO_F16 || kind == TO_BF16 ? 2 : 1;
   if (M <= 128) return 0;
   const int64_t pairs = sm_count() / 2;
@@ -437,7 +450,7 @@ int linear_pair_width(int kind, int64_t M, int64_t N) {
 // where the tiles do not apply.
 int linear_pair_launch(int kind, const LinOps& o, const LinEpi& ep, cudaStream_t st) {
   const int e = kind == TO_F16 || kind == TO_BF16 ? 2 : 1;
-  const int best = linear_pair_width(kind, o.M, o.N);
+  const int best = pair_width(kind, o.M, o.N);
   if (best == 0 || !aligned_rows(o.a, o.lda * e) || !aligned_rows(o.b, o.ldb * e))
     return TO_EUNSUPPORTED;
   const bool plain = plain_output(ep);

@@ -94,6 +94,23 @@ struct ChunkWriter {
   // turns in both slabs, so that a lane is a column and rows are read and written whole.
   __device__ __forceinline__ void put_plain(float* v, const float* bias, int col0, int row0,
                                             const LinEpi& ep, int M, int N, bool store) {
+    const int n = col0 + lane, rows = min(32, M - row0);
+    // The residual's column first: its latency passes under the activation.
+    uint32_t f[32];
+    const bool wide = dtype == TO_F32;
+    if (ep.res != nullptr && n < N) {
+      const int64_t at = (int64_t)row0 * ep.ldr + n;
+      if (wide) {
+#pragma unroll
+        for (int r = 0; r < 32; ++r) f[r] = ld_raw(ep.res, at + min(r, rows - 1) * ep.ldr, true);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 32; ++r) f[r] = ld_raw(ep.res, at + min(r, rows - 1) * ep.ldr, false);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 32; ++r) f[r] = 0u;
+    }
     finish_acts(v, bias);
     float* turn = reinterpret_cast<float*>(slab0);
     __syncwarp();  // the previous chunk has been read
@@ -102,24 +119,16 @@ struct ChunkWriter {
       *reinterpret_cast<float4*>(turn + lane * 32 + ((c ^ (lane & 7)) << 2)) =
           make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
     __syncwarp();
-    const int n = col0 + lane, rows = min(32, M - row0);
     if (n >= N || !store) return;
-#pragma unroll 1
-    for (int r0 = 0; r0 < rows; r0 += 8) {
-      float f[8];
+    const int64_t at = (int64_t)row0 * ep.ldc + n;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int r = min(r0 + u, rows - 1);
-        f[u] = ep.res != nullptr ? ld_dtype(ep.res, (int64_t)(row0 + r) * ep.ldr + n, dtype) : 0.f;
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int r = r0 + u;
-        if (r >= rows) continue;
-        const float t = turn[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
-        st_dtype(ep.c, (int64_t)(row0 + r) * ep.ldc + n, dtype, t + f[u]);
-      }
+    for (int r = 0; r < 32; ++r) {
+      const float t = turn[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
+      f[r] = __float_as_uint(t + raw_to_f32(f[r], dtype));
     }
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+      if (r < rows) st_dtype(ep.c, at + (int64_t)r * ep.ldc, dtype, __uint_as_float(f[r]));
   }
   __device__ __forceinline__ void put(float* v, const float* bias, int col0, int row0, bool store) {
     finish_acts(v, bias);

@@ -249,7 +249,7 @@ def _run_w8a8_bias_act(entry, op, a, b, a_s, b_s, block_n, block_k, m, n, k, bia
                                                       out)
     pa, pb = a.data_ptr(), b.data_ptr()
     nbytes, ws, wp = 0, None, None
-    if m > 128 and (pa | pb | k) & 15:  # rows that need aligned copies
+    if (pa | pb | k) & 15:  # rows that need aligned copies
         nbytes = _lib.load().to_w8a8_gemm_bias_act_workspace_size(pa, pb, m, n, k, block_k)
         ws, wp = _epilogue.copies(nbytes, a)
     _lib.call(entry, pa, pb, a_s.data_ptr(), b_s.data_ptr(), _lib.ptr(bias), code,
