@@ -92,25 +92,19 @@ struct ChunkWriter {
   }
   // The chunk where the output or the residual is no TMA tensor (16-byte rows, 16-bit values): it
   // turns in both slabs, so that a lane is a column and rows are read and written whole.
-  __device__ __forceinline__ void put_plain(float* v, const float* bias, int col0, int row0,
-                                            const LinEpi& ep, int M, int N, bool store) {
+  template <typename T>
+  __device__ __forceinline__ void put_rows(float* v, const float* bias, int col0, int row0,
+                                           const LinEpi& ep, int M, int N, bool store) {
     const int n = col0 + lane, rows = min(32, M - row0);
+    const bool mine = n < N && store, whole = rows == 32;
     // The residual's column first: its latency passes under the activation.
-    uint32_t f[32];
-    const bool wide = dtype == TO_F32;
-    if (ep.res != nullptr && n < N) {
-      const int64_t at = (int64_t)row0 * ep.ldr + n;
-      if (wide) {
+    T f[16];
+    const T* rp = reinterpret_cast<const T*>(ep.res) + (int64_t)row0 * ep.ldr + n;
+    auto fetch_rows = [&]() {
 #pragma unroll
-        for (int r = 0; r < 32; ++r) f[r] = ld_raw(ep.res, at + min(r, rows - 1) * ep.ldr, true);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 32; ++r) f[r] = ld_raw(ep.res, at + min(r, rows - 1) * ep.ldr, false);
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 32; ++r) f[r] = 0u;
-    }
+      for (int r = 0; r < 16; ++r, rp += ep.ldr) f[r] = *rp;
+    };
+    if (ep.res != nullptr && mine && whole) fetch_rows();
     finish_acts(v, bias);
     float* turn = reinterpret_cast<float*>(slab0);
     __syncwarp();  // the previous chunk has been read
@@ -119,16 +113,30 @@ struct ChunkWriter {
       *reinterpret_cast<float4*>(turn + lane * 32 + ((c ^ (lane & 7)) << 2)) =
           make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
     __syncwarp();
-    if (n >= N || !store) return;
-    const int64_t at = (int64_t)row0 * ep.ldc + n;
+    if (!mine) return;
+    auto at = [&](int r) { return turn[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)]; };
+    T* cp = reinterpret_cast<T*>(ep.c) + (int64_t)row0 * ep.ldc + n;
+    if (!whole) {  // the last rows
+#pragma unroll 1
+      for (int r = 0; r < rows; ++r, cp += ep.ldc, rp += ep.ldr)
+        *cp = from_f32<T>(at(r) + (ep.res != nullptr ? to_f32<T>(*rp) : 0.f));
+    } else if (ep.res != nullptr) {
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32; r0 += 16) {
+        if (r0 > 0) fetch_rows();
 #pragma unroll
-    for (int r = 0; r < 32; ++r) {
-      const float t = turn[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
-      f[r] = __float_as_uint(t + raw_to_f32(f[r], dtype));
+        for (int r = 0; r < 16; ++r, cp += ep.ldc) *cp = from_f32<T>(at(r0 + r) + to_f32<T>(f[r]));
+      }
+    } else {
+#pragma unroll 16
+      for (int r = 0; r < 32; ++r, cp += ep.ldc) *cp = from_f32<T>(at(r));
     }
-#pragma unroll
-    for (int r = 0; r < 32; ++r)
-      if (r < rows) st_dtype(ep.c, at + (int64_t)r * ep.ldc, dtype, __uint_as_float(f[r]));
+  }
+  __device__ __forceinline__ void put_plain(float* v, const float* bias, int col0, int row0,
+                                            const LinEpi& ep, int M, int N, bool store) {
+    if (dtype == TO_BF16) put_rows<__nv_bfloat16>(v, bias, col0, row0, ep, M, N, store);
+    else if (dtype == TO_F16) put_rows<__half>(v, bias, col0, row0, ep, M, N, store);
+    else put_rows<float>(v, bias, col0, row0, ep, M, N, store);
   }
   __device__ __forceinline__ void put(float* v, const float* bias, int col0, int row0, bool store) {
     finish_acts(v, bias);
