@@ -14,7 +14,7 @@ import pytest
 import torch
 
 import tileops_b200 as tob
-from tileops_b200 import _lib
+from tileops_b200 import _epilogue, _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -417,6 +417,8 @@ def test_workspace_of_the_c_entries(cuda):
     lib, f16 = _lib.load(), _lib.DTYPE_CODES[torch.float16]
     need = lib.to_gemm_bias_act_workspace_size(a.data_ptr(), k, b.data_ptr(), f16, m, n, k)
     assert need == m * 768 + k * 2048  # rows of 666 and 2002 bytes, padded to 128
+    assert need == (_epilogue.padded(m, 2 * k, a.data_ptr(), 2 * k)
+                    + _epilogue.padded(k, 2 * n, b.data_ptr(), 2 * n))
     assert lib.to_gemm_bias_act_workspace_size(1024, 336, 1024, f16, m, 1000, 333) == 0
     assert lib.to_w8a8_gemm_bias_act_workspace_size(1024, 1024, m, n, 336, 336) == 0
     assert lib.to_w8a8_gemm_bias_act_workspace_size(1024, 1024, m, n, k, k) == (m + n) * 384

@@ -67,13 +67,16 @@ def prepare(shape: tuple, n: int, like: torch.Tensor, dtype: torch.dtype,
     return bias, residual, ldr, like.new_empty(shape, dtype=dtype), n
 
 
-def copies(nbytes: int, like: torch.Tensor) -> tuple[Optional[torch.Tensor], Optional[int]]:
+def padded(rows: int, row_bytes: int, address: int, pitch: int) -> int:
+    """Bytes of the aligned copy of an operand, 0 if its rows are 16-byte aligned already; the
+    operands' sum is what the library's workspace queries return."""
+    return rows * ((row_bytes + 127) // 128 * 128) if (address | pitch) & 15 else 0
+
+
+def copies(nbytes: int, like: torch.Tensor) -> torch.Tensor:
     """Scratch for aligned copies of operands, allocated for this call alone: it can be as large as
     the weights."""
-    if nbytes == 0:
-        return None, None
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    return ws, ws.data_ptr()
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
 
 
 def finish(dst: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
@@ -83,4 +86,4 @@ def finish(dst: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
     return dst
 
 
-__all__ = ["ACT_CODES", "check", "copies", "finish", "prepare"]
+__all__ = ["ACT_CODES", "check", "copies", "finish", "padded", "prepare"]

@@ -90,12 +90,12 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
         b = b.contiguous()
     bias, residual, ldr, dst, ldc = _epilogue.prepare((m, n), n, a, dtype, bias, residual, out)
     pa, pb, dc = a.data_ptr(), b.data_ptr(), _lib.DTYPE_CODES[dtype]
-    nbytes, ws, wp = 0, None, None
-    if (pa | pb | 2 * lda | 2 * n) & 15 and dtype is not torch.float32:  # aligned copies
-        nbytes = _lib.load().to_gemm_bias_act_workspace_size(pa, lda, pb, dc, m, n, k)
-        ws, wp = _epilogue.copies(nbytes, a)
+    nbytes, ws = 0, None
+    if (pa | pb | 2 * lda | 2 * n) & 15 and dtype != torch.float32 and m and n and k:
+        nbytes = _epilogue.padded(m, 2 * k, pa, 2 * lda) + _epilogue.padded(k, 2 * n, pb, 2 * n)
+        ws = _epilogue.copies(nbytes, a)
     _lib.call("to_gemm_bias_act", pa, lda, pb, _lib.ptr(bias), code, _lib.ptr(residual), ldr,
-              dst.data_ptr(), ldc, dc, m, n, k, wp, nbytes, _lib.stream_ptr(idx))
+              dst.data_ptr(), ldc, dc, m, n, k, _lib.ptr(ws), nbytes, _lib.stream_ptr(idx))
     return _epilogue.finish(dst, out)
 
 

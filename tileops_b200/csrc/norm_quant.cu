@@ -96,50 +96,49 @@ __device__ __forceinline__ float scale_of(float maxp, float rstd, const NormArgs
   return s;
 }
 
-// The factor c of a group, rstd / s up to a few roundings: qmax / max|p|, or what the floor of the
-// scale leaves. 0 stands for the groups whose codes need a division each (a NaN or an infinity, or
-// numbers near the ends of fp32's range). Every lane works one out per pack, so it is short.
+// The factor rstd / s of a group in two terms (c, what rounding c left out): qmax / max|p|, or what
+// the floor of the scale leaves. With the second term a quotient that is a tie, half the largest
+// value say, comes out as one. (0, 0) stands for the groups whose codes need a division each (a NaN
+// or an infinity, or numbers near the ends of fp32's range).
 template <int Q>
-__device__ __forceinline__ float code_factor(float maxp, float rstd, const NormArgs& a) {
+__device__ __forceinline__ float2 code_factor(float maxp, float rstd, const NormArgs& a) {
   const float m = maxp * rstd;
-  float c = m > a.quant_eps ? __fdividef(a.qmax, maxp) : rstd * a.floor_factor;
-  if (Q == kQE4M3 && a.ue8m0) c = __fdividef(rstd, scale_of<Q>(maxp, rstd, a));
+  const bool free = m > a.quant_eps && !(Q == kQE4M3 && a.ue8m0);
+  float c = free ? __fdiv_rn(a.qmax, maxp) : rstd * a.floor_factor;
+  if (Q == kQE4M3 && a.ue8m0) c = __fdiv_rn(rstd, scale_of<Q>(maxp, rstd, a));
+  const float lo = free ? fmaf(-c, maxp, a.qmax) * (c * a.qmax_inv) : 0.f;
   const bool plain = m <= 1e30f && maxp <= 1e30f && (maxp >= 1e-30f || maxp == 0.f) &&
                      c <= 1e30f;  // false for NaN
-  return plain ? c : 0.f;
+  return plain ? make_float2(c, lo) : make_float2(0.f, 0.f);
 }
 
-// The codes of V values p c. With a factor every value is finite and |p c| <= qmax (1 + 2^-21),
+// The codes of V values p c. With a factor every value is finite and |p c| <= qmax (1 + 2^-22),
 // which saturates (e4m3) or rounds (int8) to qmax.
 template <int Q, int V>
-__device__ __forceinline__ Pack<uint8_t, V> codes_of(const Pack<float, V>& f, float c) {
+__device__ __forceinline__ Pack<uint8_t, V> codes_of(const Pack<float, V>& f, float2 c) {
   Pack<uint8_t, V> o;
+  auto z = [&](int j) { return fmaf(f.v[j], c.x, f.v[j] * c.y); };
+  // the low byte of z + 1.5 x 2^23 is rint(z)
+  auto i8 = [&](int j) { return __float_as_uint(z(j) + 12582912.0f); };
   if constexpr (V == 1) {
-    const float z = f.v[0] * c;
-    o.v[0] = Q == kQE4M3 ? f32_to_e4m3(z) : (uint8_t)__float_as_uint(z + 12582912.0f);
+    o.v[0] = Q == kQE4M3 ? f32_to_e4m3(z(0)) : (uint8_t)i8(0);
   } else if constexpr (V == 2) {
     uint16_t w;
-    if constexpr (Q == kQE4M3)
-      w = f32x2_to_e4m3x2(f.v[0] * c, f.v[1] * c);
-    else
-      w = (uint16_t)__byte_perm(__float_as_uint(fmaf(f.v[0], c, 12582912.0f)),
-                                __float_as_uint(fmaf(f.v[1], c, 12582912.0f)), 0x0040);
+    if constexpr (Q == kQE4M3) w = f32x2_to_e4m3x2(z(0), z(1));
+    else w = (uint16_t)__byte_perm(i8(0), i8(1), 0x0040);
     *reinterpret_cast<uint16_t*>(o.v) = w;
   } else {
 #pragma unroll
-    for (int k = 0; k < V / 4; ++k) {
-      const float* z = f.v + 4 * k;
+    for (int k = 0; k < V; k += 4) {
       uint32_t lo, hi;
       if constexpr (Q == kQE4M3) {
-        lo = f32x2_to_e4m3x2(z[0] * c, z[1] * c);
-        hi = f32x2_to_e4m3x2(z[2] * c, z[3] * c);
-      } else {  // the low byte of z + 1.5 x 2^23 is rint(z)
-        lo = __byte_perm(__float_as_uint(fmaf(z[0], c, 12582912.0f)),
-                         __float_as_uint(fmaf(z[1], c, 12582912.0f)), 0x0040);
-        hi = __byte_perm(__float_as_uint(fmaf(z[2], c, 12582912.0f)),
-                         __float_as_uint(fmaf(z[3], c, 12582912.0f)), 0x0040);
+        lo = f32x2_to_e4m3x2(z(k), z(k + 1));
+        hi = f32x2_to_e4m3x2(z(k + 2), z(k + 3));
+      } else {
+        lo = __byte_perm(i8(k), i8(k + 1), 0x0040);
+        hi = __byte_perm(i8(k + 2), i8(k + 3), 0x0040);
       }
-      reinterpret_cast<uint32_t*>(o.v)[k] = __byte_perm(lo, hi, 0x5410);
+      reinterpret_cast<uint32_t*>(o.v)[k / 4] = __byte_perm(lo, hi, 0x5410);
     }
   }
   return o;
@@ -295,9 +294,9 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlocksMin<V, MAXV>)
     else scales[g] = s;
   };
   // Codes of a pack whose group has the maximum maxp.
-  auto emit = [&](int v, const F& f, float maxp, float c) {
+  auto emit = [&](int v, const F& f, float maxp, float2 c) {
     Pack<uint8_t, V> o;
-    if (c != 0.f) {
+    if (c.x != 0.f) {
       o = codes_of<Q, V>(f, c);
     } else {
       const float s = scale_of<Q>(maxp, rstd, a);
@@ -336,10 +335,11 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlocksMin<V, MAXV>)
       const int v_mine = tid + i_mine * team;
       if (active && i_mine < MAXV && v_mine < nvec)
         put_scale(v_mine >> shift, scale_of<Q>(mine, rstd, a));
-      const float c = code_factor<Q>(mine, rstd, a);
+      const float2 c = code_factor<Q>(mine, rstd, a);
 #pragma unroll
       for (int i = 0; i < MAXV; ++i) {
-        const float ci = __shfl_sync(0xffffffffu, c, lane - i_mine + i);
+        const float2 ci = make_float2(__shfl_sync(0xffffffffu, c.x, lane - i_mine + i),
+                                      __shfl_sync(0xffffffffu, c.y, lane - i_mine + i));
         if (active && tid + i * team < nvec) emit(tid + i * team, y[i], m[i], ci);
       }
     } else {
@@ -382,7 +382,8 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlocksMin<V, MAXV>)
       for (int g = tid; active && g < groups; g += team)
         put_scale(g, scale_of<Q>(__uint_as_float(gm[g]), rstd, a));
     }
-    const float c_row = MODE == kGroupRow ? code_factor<Q>(rowmax, rstd, a) : 0.f;
+    const float2 c_row =
+        MODE == kGroupRow ? code_factor<Q>(rowmax, rstd, a) : make_float2(0.f, 0.f);
     auto finish = [&](int v, const F& f) {
       if constexpr (MODE == kGroupRow) {
         emit(v, f, rowmax, c_row);

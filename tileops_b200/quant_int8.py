@@ -248,13 +248,13 @@ def _run_w8a8_bias_act(entry, op, a, b, a_s, b_s, block_n, block_k, m, n, k, bia
     bias, residual, ldr, dst, ldc = _epilogue.prepare(shape, n, a, output_dtype, bias, residual,
                                                       out)
     pa, pb = a.data_ptr(), b.data_ptr()
-    nbytes, ws, wp = 0, None, None
-    if (pa | pb | k) & 15:  # rows that need aligned copies
-        nbytes = _lib.load().to_w8a8_gemm_bias_act_workspace_size(pa, pb, m, n, k, block_k)
-        ws, wp = _epilogue.copies(nbytes, a)
+    nbytes, ws = 0, None
+    if (pa | pb | k) & 15 and m and n and (block_k >= k or block_k % 128 == 0):
+        nbytes = _epilogue.padded(m, k, pa, k) + _epilogue.padded(n, k, pb, k)
+        ws = _epilogue.copies(nbytes, a)
     _lib.call(entry, pa, pb, a_s.data_ptr(), b_s.data_ptr(), _lib.ptr(bias), code,
               _lib.ptr(residual), ldr, dst.data_ptr(), ldc, _lib.DTYPE_CODES[output_dtype], m, n,
-              k, block_n, block_k, wp, nbytes, _lib.stream_ptr(idx))
+              k, block_n, block_k, _lib.ptr(ws), nbytes, _lib.stream_ptr(idx))
     return _epilogue.finish(dst, out)
 
 
