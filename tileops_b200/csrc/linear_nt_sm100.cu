@@ -166,34 +166,41 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS>::kThreads,
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc =
-          make_idesc_major(Tr::kDFmt, Tr::kAFmt, Tr::kBFmt, 128, NT, C::kMn ? 1 : 0, 0);
-      bool any = false;
-      for (int it = 0; it < kb_n; ++it) {
-        const int s = it % ST;
-        if (!mbar_wait_polled(full + s, (uint32_t)(it / ST) & 1u, abort_flag, err)) { ok = false; break; }
-        const int b = BS ? it & 1 : 0;
-        if (BS && it >= 2 &&
-            !mbar_wait_polled(tempty + b, ((uint32_t)(it >> 1) & 1u) ^ 1, abort_flag, err)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t w0 = smem_u32(sW + (size_t)s * C::kWBytes);
-        const uint32_t x0 = smem_u32(sX + (size_t)s * C::kXBytes);
+    // The whole warp walks the loop and one lane issues, so that addresses and descriptors stay in
+    // uniform registers: per lane, their arithmetic bounds the slices of a split product.
+    constexpr uint32_t idesc =
+        make_idesc_major(Tr::kDFmt, Tr::kAFmt, Tr::kBFmt, 128, NT, C::kMn ? 1 : 0, 0);
+    // MN-major: 64-column strips of 64 K rows (8 KB apart); 16 K rows are 2 KB
+    constexpr uint32_t kWStep = (C::kMn ? 2048 : 32) >> 4;
+    const uint64_t wdesc = C::kMn ? smem_desc_mnmajor_sw128(smem_u32(sW), 8192, 1024)
+                                  : smem_desc_kmajor_sw128(smem_u32(sW));
+    const uint64_t xdesc = smem_desc_kmajor_sw128(smem_u32(sX));
+    const bool issue = elect_one();
+    bool any = false;
+    int s = 0;
+    uint32_t ph = 0;
+    for (int it = 0; it < kb_n; ++it) {
+      const int b = BS ? it & 1 : 0;
+      ok = mbar_wait_warp(full + s, ph, abort_flag, err);
+      if (BS && ok && it >= 2)
+        ok = mbar_wait_warp(tempty + b, ((uint32_t)(it >> 1) & 1u) ^ 1, abort_flag, err);
+      if (!ok) break;
+      tc_fence_after();
+      if (issue) {
+        const uint64_t wd = wdesc + (uint64_t)(s * (C::kWBytes >> 4));
+        const uint64_t xd = xdesc + (uint64_t)(s * (C::kXBytes >> 4));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          // MN-major: 64-column strips of 64 K rows (8 KB apart); 16 K rows are 2 KB
-          const uint64_t wd = C::kMn ? smem_desc_mnmajor_sw128(w0 + 2048 * k, 8192, 1024)
-                                     : smem_desc_kmajor_sw128(w0 + 32 * k);
-          umma<KD>(tmem + (uint32_t)(b * NT), wd, smem_desc_kmajor_sw128(x0 + 32 * k), idesc,
+        for (int k = 0; k < 4; ++k)
+          umma<KD>(tmem + (uint32_t)(b * NT), wd + kWStep * k, xd + 2 * k, idesc,
                    BS ? k != 0 : (it | k) != 0);
-        }
-        any = true;
         umma_commit(empty + s);
         if (BS) umma_commit(tfull + b);
       }
+      __syncwarp();
+      any = true;
+      if (++s == ST) { s = 0; ph ^= 1; }
+    }
+    if (issue) {
       if (ok && !BS) umma_commit(tfull);
       if (!ok && any) {
         // Unwinding: wait (bounded) until the MMAs already issued have finished with TMEM.
@@ -203,6 +210,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS>::kThreads,
         }
       }
     }
+    __syncwarp();
   }
 
   // -------------------------------------------------------------- epilogue
@@ -239,17 +247,28 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS>::kThreads,
     if (!BS && ep.b_s != nullptr && n_ok) sb = __ldg(ep.b_s + brow);
     const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * C::kTpt);
     if constexpr (BS) {
-      float run[C::kTpt], sa_l[(C::kTpt + 31) / 32];
+      // A slice's scales are loaded while the one before is folded: their latency is as long as a
+      // slice of few tokens.
+      constexpr int kSa = (C::kTpt + 31) / 32;
+      float run[C::kTpt], sa_n[kSa], s_col_n = 0.f;
 #pragma unroll
       for (int j = 0; j < C::kTpt; ++j) run[j] = 0.f;
-      for (int it = 0; it < kb_n; ++it) {
+      auto load_scales = [&](int it) {
         const int kb = (kb_lo + it) / ep.kb_per_scale;
-        const float s_col = n_ok ? __ldg(ep.b_s + brow + kb) : 0.f;
+        s_col_n = n_ok ? __ldg(ep.b_s + brow + kb) : 0.f;
 #pragma unroll
-        for (int i = 0; i < (C::kTpt + 31) / 32; ++i) {
+        for (int i = 0; i < kSa; ++i) {
           const int t = half * C::kTpt + i * 32 + lane;
-          sa_l[i] = t < tokens ? __ldg(ep.a_s + (int64_t)(t0 + t) * ep.a_s_ld + kb) : 0.f;
+          sa_n[i] = t < tokens ? __ldg(ep.a_s + (int64_t)(t0 + t) * ep.a_s_ld + kb) : 0.f;
         }
+      };
+      if (kb_n > 0) load_scales(0);
+      for (int it = 0; it < kb_n; ++it) {
+        const float s_col = s_col_n;
+        float sa_l[kSa];
+#pragma unroll
+        for (int i = 0; i < kSa; ++i) sa_l[i] = sa_n[i];
+        if (it + 1 < kb_n) load_scales(it + 1);
         const int b = it & 1;
         if (!mbar_wait_polled(tfull + b, (uint32_t)(it >> 1) & 1u, abort_flag, err)) { ok = false; break; }
         tc_fence_after();
