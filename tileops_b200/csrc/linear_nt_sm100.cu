@@ -443,23 +443,34 @@ int clusters_at_once(const void* kern, int threads, size_t smem, int per_sm, int
   return n[S];
 }
 
+// K split: the most CTAs that the SMs hold at once, at least two K blocks each, at most a portable
+// cluster of eight. Clusters have to fit into the GPU's processor clusters whole, so the count comes
+// from the driver. One token, 7168 x 7168 FP8 block-scaled, 56 tiles: two ways 21.6 us, three 16.3,
+// four 14.1, and five, 280 CTAs for 296 places but two rounds, 20.0. 0: not even unsplit.
+template <Kind KD, int NT, bool BS>
+int split_of(const LinOps& o) {
+  using C = NtCfg<KD, NT, BS>;
+  const void* kern = (const void*)k_linear_nt<KD, NT, BS>;
+  const int64_t tiles = ceil_div(o.N, 128) * ceil_div(o.M, NT);
+  int S = (int)std::min<int64_t>(8, std::max<int64_t>(1, ceil_div(o.K, C::kBK) / 2));
+  while (S > 0 && tiles > clusters_at_once(kern, C::kThreads, C::kSmem, C::kMinBlocks, S)) --S;
+  return S;
+}
+
+template <Kind KD, int NT, bool BS>
+cudaError_t set_smem() {
+  return ensure_smem_attr((const void*)k_linear_nt<KD, NT, BS>, (int)NtCfg<KD, NT, BS>::kSmem);
+}
+
 template <Kind KD, int NT, bool BS>
 int launch_nt(const LinOps& o, const LinEpi& ep, cudaStream_t st) {
   using C = NtCfg<KD, NT, BS>;
   auto kern = k_linear_nt<KD, NT, BS>;
-  const cudaError_t ae = ensure_smem_attr((const void*)kern, (int)C::kSmem);
+  const cudaError_t ae = set_smem<KD, NT, BS>();
   if (ae != cudaSuccess) return cuda_fail(ae, "linear epilogue: shared memory attribute");
   const int64_t M = o.M, N = o.N, K = o.K;
   const int64_t n_tiles = ceil_div(N, 128), m_tiles = ceil_div(M, NT);
-  const int64_t kblocks = ceil_div(K, C::kBK);
-  // K split: the most CTAs that the SMs hold at once, at least two K blocks each, at most a portable
-  // cluster of eight. Clusters have to fit into the GPU's processor clusters whole, so the count
-  // comes from the driver. One token, 7168 x 7168 FP8 block-scaled, 56 tiles: two ways 21.6 us, three
-  // 16.3, four 14.1, and five, 280 CTAs for 296 places but two rounds, 20.0.
-  int64_t S = std::min<int64_t>(8, std::max<int64_t>(1, kblocks / 2));
-  while (S > 1 && n_tiles * m_tiles > clusters_at_once((const void*)kern, C::kThreads, C::kSmem,
-                                                       C::kMinBlocks, (int)S))
-    --S;
+  const int64_t S = std::max(1, split_of<KD, NT, BS>(o));
   if (n_tiles * S > INT32_MAX || m_tiles > 65535)
     return fail(TO_EUNSUPPORTED, "linear epilogue: too many tiles (M=%lld N=%lld)", (long long)M,
                 (long long)N);
@@ -507,6 +518,15 @@ int launch_nt_any(const LinOps& o, const LinEpi& ep, cudaStream_t st) {
       1, std::min<int64_t>(8, ceil_div(K * KindTraits<KD>::kElemBytes, 128) / 2));
   int nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   while (nt > 16 && n_tiles * ceil_div(M, nt) * split < sm_count()) nt /= 2;
+  // 64 tokens wide, an SM holds two CTAs: better where that lets K split further (145 tokens, 12544
+  // -> 2240 bf16: 33.4 us three ways at 128, 25.9 four ways at 64), or where a CTA's K is short and
+  // one's start and end pass under the other's loads (128 tokens, 1024 -> 7168: 14.7 and 11.7 us).
+  // On long K the weights read twice cost more (80 tokens, 8192 -> 14336: 58 and 64 us).
+  if (nt == 128 && set_smem<KD, 128, BS>() == cudaSuccess && set_smem<KD, 64, BS>() == cudaSuccess) {
+    const int s128 = std::max(1, split_of<KD, 128, BS>(o)), s64 = split_of<KD, 64, BS>(o);
+    const int64_t blocks = ceil_div(K * KindTraits<KD>::kElemBytes, 128);
+    if (s64 > s128 || (s64 == s128 && blocks <= 32 * s64)) nt = 64;
+  }
   if (nt == 16) return launch_nt<KD, 16, BS>(o, ep, st);
   if (nt == 32) return launch_nt<KD, 32, BS>(o, ep, st);
   if (nt == 64) return launch_nt<KD, 64, BS>(o, ep, st);
