@@ -115,6 +115,16 @@ def test_w8a8_exact(cuda, codes, scales, m, n, k):
         assert torch.equal(y, want), (dt, list(kw))
 
 
+@pytest.mark.parametrize("m,n,k", [(65, 9600, 96), (80, 20000, 64), (128, 7200, 160),
+                                   (145, 2240, 1300), (162, 3520, 1280), (129, 190, 2100)])
+def test_tile_choices(cuda, m, n, k):
+    """Half-empty pairs of wide outputs, and few tiles of some more than 64 tokens with K split."""
+    test_dense_exact(cuda, torch.bfloat16, m, n, k)
+    for codes in ("int8", "e4m3"):
+        for scales in ("channel", "block128", "odd_n"):
+            test_w8a8_exact(cuda, codes, scales, m, n, k)
+
+
 @pytest.mark.parametrize("act", [None, "relu", "silu", "gelu"])
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("m,n,k", [(1, 512, 1024), (40, 333, 777), (300, 1024, 512)])

@@ -520,8 +520,9 @@ int launch_nt_any(const LinOps& o, const LinEpi& ep, cudaStream_t st) {
   while (nt > 16 && n_tiles * ceil_div(M, nt) * split < sm_count()) nt /= 2;
   // 64 tokens wide, an SM holds two CTAs: better where that lets K split further (145 tokens, 12544
   // -> 2240 bf16: 33.4 us three ways at 128, 25.9 four ways at 64), or where a CTA's K is short and
-  // one's start and end pass under the other's loads (128 tokens, 1024 -> 7168: 14.7 and 11.7 us).
-  // On long K the weights read twice cost more (80 tokens, 8192 -> 14336: 58 and 64 us).
+  // one's start and end pass under the other's loads (128 tokens, 1024 -> 4096: 10.2 and 8.7 us;
+  // 200 tokens, 4096 -> 4096: 23.0 and 20.7). On long K the weights read twice cost more (80 tokens,
+  // 8192 -> 4096, at the limit of 32: 18.8 and 20.0).
   if (nt == 128 && set_smem<KD, 128, BS>() == cudaSuccess && set_smem<KD, 64, BS>() == cudaSuccess) {
     const int s128 = std::max(1, split_of<KD, 128, BS>(o)), s64 = split_of<KD, 64, BS>(o);
     const int64_t blocks = ceil_div(K * KindTraits<KD>::kElemBytes, 128);

@@ -427,7 +427,10 @@ int launch_pair(const LinOps& o, bool plain_out, const LinEpi& ep, cudaStream_t 
 // SMs without splitting K). Operands have to be of 16-byte aligned rows.
 static int pair_width(int kind, int64_t M, int64_t N) {
   const int e = kind == TO_F16 || kind == TO_BF16 ? 2 : 1;
-  if (M <= 128) return 0;
+  // Up to 64 tokens the weights-as-rows tiles waste less (64 tokens, 8192 -> 28672 bf16: 78.7 us
+  // there, 94.4 here); above, the pairs win although half their rows may be empty (80 tokens: 119 and
+  // 96; 1024 -> 28672: 39.2 and 18.1; FP8, 8192 -> 14336: 39.1 and 30.4).
+  if (M <= 64) return 0;
   const int64_t pairs = sm_count() / 2;
   // Tile width: the one whose rounds of tiles cost least; a tile's time is its width plus a fixed
   // part worth about 32 columns.
