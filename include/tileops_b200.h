@@ -365,7 +365,7 @@ TO_API int to_act_and_mul_group_quant(const void* a, const void* b, int dtype, i
 /* Library extension (no reference counterpart): residual add, root-mean-square norm and per-group
  * quantisation of [rows, cols] in one pass: h = x + residual (residual may be NULL), y = h /
  * sqrt(mean(h^2) + eps) * weight, scale = max(max|y|, quant_eps) / qmax per group of group_size
- * columns (group_size divides cols; q_dtype TO_E4M3: qmax 448, ue8m0 and column_major as
+ * columns (group_size divides cols; eps >= 0, quant_eps >= 1e-35; q_dtype TO_E4M3: qmax 448, ue8m0 and column_major as
  * to_per_token_group_quant_fp8; TO_I8: 127), q [rows, cols] the codes of y / scale, dense. fp32
  * throughout; y is not rounded to dtype. h rounded to dtype goes to residual_out, given exactly
  * when residual is (x or residual itself allowed). x, residual, residual_out rows ldx, ldr, ldh apart; weight

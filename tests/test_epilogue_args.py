@@ -77,6 +77,11 @@ def test_fnuz_operands_are_refused():
     (TypeError, "weight.dtype", (Z(2, 8), Z(8).half(), 4), {}),
     (ValueError, "needs a residual", (Z(2, 8), Z(8), 4), {"residual_out": Z(2, 8)}),
     (ValueError, "residual_out.shape", (Z(2, 8), Z(8), 4, Z(2, 8)), {"residual_out": Z(8, 2)}),
+    (ValueError, "quant_eps", (Z(2, 8), Z(8), 4), {"quant_eps": 0.0}),
+    (ValueError, "quant_eps", (Z(2, 8), Z(8), 4), {"quant_eps": float("nan")}),
+    (ValueError, "quant_eps", (Z(2, 8), Z(8), 4), {"quant_eps": float("inf")}),
+    (ValueError, "eps", (Z(2, 8), Z(8), 4), {"eps": -1e-6}),
+    (ValueError, "eps", (Z(2, 8), Z(8), 4), {"eps": float("nan")}),
     (TypeError, "CUDA", (Z(2, 8), Z(8), 4), {}),
 ])
 def test_norm_quant_refusals(err, match, args, kw):
@@ -105,11 +110,14 @@ def test_c_entries_check_before_they_launch():
         assert w8a8(0, 2, 8) == _lib.TO_OK
         assert w8a8(2, 2, 8, act=-1) == _lib.TO_EINVAL and w8a8(2, 2, 8, p=None) == _lib.TO_EINVAL
 
-    def norm(rows, cols, g, qd=torch.int8, ue=0, ldx=8, p=1 << 20):
-        return lib.to_add_rms_norm_group_quant(p, ldx, None, 0, p, f16, rows, cols, g, 1e-6, 1e-10,
+    def norm(rows, cols, g, qd=torch.int8, ue=0, ldx=8, p=1 << 20, eps=1e-6, qe=1e-10):
+        return lib.to_add_rms_norm_group_quant(p, ldx, None, 0, p, f16, rows, cols, g, eps, qe,
                                                ue, 0, _lib.DTYPE_CODES[qd], p, p, None, 0, None)
 
     assert norm(2, 8, 3) == _lib.TO_EINVAL and norm(2, 8, 0) == _lib.TO_EINVAL
     assert norm(2, 8, 8, ldx=4) == _lib.TO_EINVAL and norm(2, 8, 8, ue=1) == _lib.TO_EINVAL
     assert norm(2, 8, 8, qd=torch.float16) == _lib.TO_EUNSUPPORTED
+    nan = float("nan")
+    assert norm(2, 8, 8, qe=0.0) == _lib.TO_EINVAL and norm(2, 8, 8, qe=nan) == _lib.TO_EINVAL
+    assert norm(2, 8, 8, eps=-1.0) == _lib.TO_EINVAL and norm(2, 8, 8, eps=nan) == _lib.TO_EINVAL
     assert norm(0, 8, 8) == _lib.TO_OK and norm(2, 8, 8, p=None) == _lib.TO_EINVAL

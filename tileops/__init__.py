@@ -2,8 +2,10 @@
 ``import tileops.quant_awq`` resolve to the sm_100a implementation in :mod:`tileops_b200`.
 Only the quantized-linear modules, the gated activations of ``tileops.fused``
 (``silu_and_mul``, ``gelu_and_mul``) and the dense ``gemm`` / ``mm`` / ``gemv`` / ``mv``
-comparators are provided (also as ``tileops.blas``); the rest of the reference package (other
-elementwise ops, norms, attention, other BLAS, Metal backends) is not part of this library."""
+comparators are provided (also as ``tileops.blas``), with this library's own fused forms beside
+them (``add_rms_norm_group_quant``, ``gemm_bias_act``, ``w8a8_block_*_matmul_bias_act``); the rest
+of the reference package (other elementwise ops, its norms, attention, other BLAS, Metal backends)
+is not part of this library."""
 
 import sys as _sys
 

@@ -12,6 +12,10 @@
 // microsecond, and signals that cross SMs cost more than that. Wide tiles nearly halve the
 // operand bytes per product against 128 x 128 (44 KB per slice and 128 x 224 results).
 //
+// Bound by shared memory: a slice's 44 KB are written by the copies and read by the MMAs, 88 KB at
+// 128 B a clock, 700 clocks for MMAs of 450. 4096 x 7168 x 7168 FP8 with a residual: 242 us in a lone
+// launch, 1.74 PFLOP/s, and 283 us back to back (power cap); on CTA pairs it was 442 us.
+//
 // Every wait is bounded (kWaitLimitNs).
 #include <string.h>
 

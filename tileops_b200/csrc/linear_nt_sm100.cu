@@ -15,6 +15,11 @@
 //
 // Operands come by TMA: their rows are 16-byte aligned, by themselves or as padded copies.
 //
+// Graph-timed on inputs beyond L2 (floor: the bytes at the copy rate of 6.45 TB/s): bf16 4096 x 4096,
+// one token 8.5 us (5.2); bf16 14336 -> 4096, 16 tokens 21.7 us (18.3), 5.4 TB/s; FP8 8192 -> 28672, one
+// token 39.9 us (36.4), 5.9 TB/s; FP8 block-scaled 7168 x 7168, one token 12.3 us (8.0). What is left of
+// the short ones is a launch, the first copy's latency and the cluster's barrier, 3 to 4 us.
+//
 // Roles: warp 0 weight copies, warp 1 MMA issue and TMEM, warp 2 token copies, warp 3 idle, then
 // kEpiWarps epilogue warps (lane quarter = warp % 4).
 // Every wait is bounded (kWaitLimitNs); on expiry all roles unwind through the same barriers.
@@ -23,9 +28,7 @@
 #include <string.h>
 
 #include <algorithm>
-#include <array>
-#include <map>
-#include <mutex>
+#include <atomic>
 #include <type_traits>
 
 #include "linear_epi.cuh"
@@ -409,38 +412,41 @@ int strips_map(CUtensorMap* out, const void* p, int64_t K, int64_t N, int64_t pi
   return TO_OK;
 }
 
-// Clusters of S blocks of `kern`, made for per_sm blocks of an SM, that the current device runs at
-// once (asked once per kernel and device; 0 if the driver cannot say).
-int clusters_at_once(const void* kern, int threads, size_t smem, int per_sm, int S) {
-  static std::mutex mu;
-  static std::map<std::pair<const void*, int>, std::array<int, 9>> known;
+// Clusters of S (at most 8) CTAs that the current device holds at once: the driver's count, asked once
+// per device and kernel. Threads that ask at the same time store the same number.
+template <Kind KD, int NT, bool BS>
+int clusters_at_once(int S) {
+  using C = NtCfg<KD, NT, BS>;
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices][9];  // count + 1, 0 unknown
+  const void* kern = (const void*)k_linear_nt<KD, NT, BS>;
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  std::lock_guard<std::mutex> lock(mu);
-  std::array<int, 9>& n = known.try_emplace({kern, dev}, std::array<int, 9>{}).first->second;
-  if (n[0] == 0) {
-    for (int s = 1; s <= 8; ++s) {
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3((unsigned)(s * 1024), 1, 1);
-      cfg.blockDim = dim3((unsigned)threads, 1, 1);
-      cfg.dynamicSmemBytes = smem;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = (unsigned)s;
-      attr[0].val.clusterDim.y = 1;
-      attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      int count = 0;
-      n[s] = cudaOccupancyMaxActiveClusters(&count, kern, &cfg) == cudaSuccess ? count : 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return 0;
+  auto ask = [&](int s) {
+    int n = known[dev][s].load(std::memory_order_relaxed);
+    if (n > 0) return n - 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(s * 1024), 1, 1);
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)s;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+      (void)cudaGetLastError();  // the launch itself says what is wrong
+      return 0;
     }
-    // The driver counts one block per SM; the kernels sized for two run two (their blocks were seen
-    // to start together, and the split that this count allows is the fastest).
-    const int times = n[1] <= sm_count() ? per_sm : 1;
-    for (int s = 1; s <= 8; ++s) n[s] *= times;
-    n[0] = 1;
-  }
-  return n[S];
+    known[dev][s].store(n + 1, std::memory_order_relaxed);
+    return n;
+  };
+  // The driver counts one block per SM; the kernels sized for two run two (their blocks were seen to
+  // start together, and the split that this count allows is the fastest).
+  const int times = ask(1) <= sm_count() ? C::kMinBlocks : 1;
+  return ask(S) * times;
 }
 
 // K split: the most CTAs that the SMs hold at once, at least two K blocks each, at most a portable
@@ -449,11 +455,9 @@ int clusters_at_once(const void* kern, int threads, size_t smem, int per_sm, int
 // four 14.1, and five, 280 CTAs for 296 places but two rounds, 20.0. 0: not even unsplit.
 template <Kind KD, int NT, bool BS>
 int split_of(const LinOps& o) {
-  using C = NtCfg<KD, NT, BS>;
-  const void* kern = (const void*)k_linear_nt<KD, NT, BS>;
   const int64_t tiles = ceil_div(o.N, 128) * ceil_div(o.M, NT);
-  int S = (int)std::min<int64_t>(8, std::max<int64_t>(1, ceil_div(o.K, C::kBK) / 2));
-  while (S > 0 && tiles > clusters_at_once(kern, C::kThreads, C::kSmem, C::kMinBlocks, S)) --S;
+  int S = (int)std::min<int64_t>(8, std::max<int64_t>(1, ceil_div(o.K, NtCfg<KD, NT, BS>::kBK) / 2));
+  while (S > 0 && tiles > clusters_at_once<KD, NT, BS>(S)) --S;
   return S;
 }
 

@@ -13,6 +13,11 @@
 // The residual arrives by TMA in the slab of shared memory its chunk's result leaves from, one
 // chunk ahead of its use; results leave by TMA stores.
 //
+// Bound by the tensor cores under the power cap: 2048 x 8192 x 28672 bf16 with bias and gelu 743 us,
+// 1.29 PFLOP/s (1.40 sustained by a plain library product); FP8 8192^3 with bias, gelu and residual
+// 438 us, 2.51 PFLOP/s. Between 65 and some 1000 tokens, by the operands through L2: 512 tokens of FP8
+// 7168 -> 2048 15 us, 128 tokens of bf16 1024 -> 28672 18 us.
+//
 // Roles: warp 0 copies of A, warp 1 MMA issue (leader CTA) and TMEM, warps 2..9 epilogue (two per
 // TMEM lane quarter), warp 10 copies of B. Every wait is bounded (kWaitLimitNs).
 #include <string.h>

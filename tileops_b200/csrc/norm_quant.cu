@@ -162,7 +162,8 @@ template <int V, int MAXV> constexpr int kBlocksMin = V * MAXV >= 16 ? 2 : 1;
 // One block per rows_per_block rows, a team of threads each. RES: with a residual and its output.
 // Loads are not guarded but clamped (rows and packs past the end re-read the last and count as
 // zero), so that all of a thread's loads go out together. 8192 x 8192 bf16 -> e4m3 with residual:
-// 87 us, 5.4 TB/s; a persistent form fed by bulk copies into shared memory ran no faster.
+// 76 us, 6.2 TB/s (floor at the copy rate 73); a persistent form fed by bulk copies into shared memory
+// ran no faster.
 template <typename T, int Q, int V, int MAXV, int MODE, bool RES>
 __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlocksMin<V, MAXV>)
     k_norm_quant(const __grid_constant__ NormArgs a) {
@@ -503,6 +504,9 @@ extern "C" int to_add_rms_norm_group_quant(
     return fail(TO_EINVAL, "%s: invalid shape rows=%lld cols=%lld group=%lld strides=(%lld, %lld, "
                 "%lld)", op, (long long)rows, (long long)cols, (long long)group_size,
                 (long long)ldx, (long long)ldr, (long long)ldh);
+  if (!(quant_eps >= 1e-35f && quant_eps < 3e38f) || !(eps >= 0.0f && eps < 3e38f))
+    return fail(TO_EINVAL, "%s: eps=%g must be at least 0, quant_eps=%g at least 1e-35", op,
+                (double)eps, (double)quant_eps);
   if (q_dtype != TO_E4M3 && q_dtype != TO_I8)
     return fail(TO_EUNSUPPORTED, "%s: codes %s (float8_e4m3fn or int8)", op, dtype_name(q_dtype));
   if (q_dtype == TO_I8 && (ue8m0 || column_major))

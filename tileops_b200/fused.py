@@ -177,7 +177,7 @@ def add_rms_norm_group_quant(x: torch.Tensor, weight: torch.Tensor, group_size: 
     Returns ``(q, scales)``, or ``(q, scales, h)`` with a residual, h rounded to ``x.dtype``:
     written to ``residual_out`` when given, which may be ``x`` or ``residual`` itself. A row with
     a NaN has NaN scales, e4m3 NaN codes and int8 zeros; a row of zeros has codes 0 and scales
-    quant_eps / qmax."""
+    quant_eps / qmax (with ``eps`` 0 it is 0 / 0: NaN)."""
     op = "add_rms_norm_group_quant"
     if x.dim() == 0 or weight.shape != x.shape[-1:]:
         raise ValueError(f"{op}: weight.shape={tuple(weight.shape)} does not match the last "
@@ -186,6 +186,9 @@ def add_rms_norm_group_quant(x: torch.Tensor, weight: torch.Tensor, group_size: 
     if group_size <= 0 or cols % group_size != 0:
         raise ValueError(f"{op}: the last dimension of `x` {cols} must be divisible by "
                          f"`group_size` {group_size}")
+    if not (1e-35 <= quant_eps < 3e38) or not 0.0 <= eps < 3e38:
+        raise ValueError(f"{op}: eps={eps} must be at least 0 and quant_eps={quant_eps} at least "
+                         "1e-35 (a scale is a normal number)")
     if dtype is None:
         dtype = torch.float8_e4m3fn
     code = 4 if dtype == torch.float8_e4m3fn else 3
