@@ -10,8 +10,9 @@
 // 128 x 256 x 128-byte step, which L2 delivers at the tensor cores' rate (a 128 x 128 tile per CTA
 // needs twice that and was bound by it).
 //
-// The residual arrives by TMA in the slab of shared memory its chunk's result leaves from, one
-// chunk ahead of its use; results leave by TMA stores.
+// The residual arrives by TMA in the slab of shared memory its chunk's result leaves from, two
+// chunks ahead of its use; results leave by TMA stores. (Turned by generic stores and written in
+// 16-byte pieces instead, 4096 x 512 -> 4096 FP8 with residual took 36 us instead of 28.)
 //
 // Bound by the tensor cores under the power cap: 2048 x 8192 x 28672 bf16 with bias and gelu 743 us,
 // 1.29 PFLOP/s (1.40 sustained by a plain library product); FP8 8192^3 with bias, gelu and residual

@@ -12,6 +12,8 @@
 // shuffles where a group is a power-of-two number of packs within a warp, the team's reduction
 // (with the sum's) where it is the row, and shared-memory maxima (order-independent) for any other
 // group size. Few rows take one or two packs per thread: their time is the latency of one load.
+#include <string.h>
+
 #include <algorithm>
 
 #include "quant_codes.cuh"
@@ -37,6 +39,43 @@ struct NormArgs {
   int ue8m0;
   ScaleLayout sl;
 };
+
+// Data that pass once: x and r are not read again, h and the codes not before another kernel. Marked
+// to leave L2 first, they do not push one another out (8192 x 8192 back to back: 88 us unmarked,
+// 80.5 with loads and stores marked, 81 with the stores alone; a product that follows reads the codes
+// as fast).
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> ld_once(const T* p) {
+  Pack<T, V> o;
+  if constexpr (sizeof(o) == 16) {
+    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+    memcpy(&o, &u, 16);
+  } else if constexpr (sizeof(o) == 8) {
+    const uint2 u = __ldcs(reinterpret_cast<const uint2*>(p));
+    memcpy(&o, &u, 8);
+  } else {
+    o = ld_pack<T, V>(p);
+  }
+  return o;
+}
+template <typename T, int V>
+__device__ __forceinline__ void st_once(T* p, const Pack<T, V>& v) {
+  if constexpr (sizeof(v) == 16) {
+    uint4 u;
+    memcpy(&u, &v, 16);
+    __stcs(reinterpret_cast<uint4*>(p), u);
+  } else if constexpr (sizeof(v) == 8) {
+    uint2 u;
+    memcpy(&u, &v, 8);
+    __stcs(reinterpret_cast<uint2*>(p), u);
+  } else if constexpr (sizeof(v) == 4) {
+    unsigned u;
+    memcpy(&u, &v, 4);
+    __stcs(reinterpret_cast<unsigned*>(p), u);
+  } else {
+    st_pack<T, V>(p, v);
+  }
+}
 
 // max(|v|, m), NaN when either is.
 __device__ __forceinline__ float max_abs_nan(float v, float m) {
@@ -162,8 +201,8 @@ template <int V, int MAXV> constexpr int kBlocksMin = V * MAXV >= 16 ? 2 : 1;
 // One block per rows_per_block rows, a team of threads each. RES: with a residual and its output.
 // Loads are not guarded but clamped (rows and packs past the end re-read the last and count as
 // zero), so that all of a thread's loads go out together. 8192 x 8192 bf16 -> e4m3 with residual:
-// 76 us in a lone launch, 88 back to back, 5.4 TB/s (floor at the copy rate 73); a persistent form fed
-// by bulk copies into shared memory ran no faster.
+// 80.5 us back to back, 5.9 TB/s (floor at the copy rate 73); a persistent form fed by bulk copies into
+// shared memory ran no faster.
 template <typename T, int Q, int V, int MAXV, int MODE, bool RES>
 __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlocksMin<V, MAXV>)
     k_norm_quant(const __grid_constant__ NormArgs a) {
@@ -205,7 +244,7 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlocksMin<V, MAXV>)
 #pragma unroll
         for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(f.v[j]);
       }
-      st_pack<T, V>(h + (int64_t)v * V, o);
+      st_once<T, V>(h + (int64_t)v * V, o);
     }
   };
   auto load_h = [&](int v) {
@@ -236,8 +275,8 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlocksMin<V, MAXV>)
 #pragma unroll
     for (int i = 0; i < MAXV; ++i) {
       const int v = min(tid + i * team, nvec - 1);
-      px[i] = ld_pack<T, V>(x + (int64_t)v * V);
-      if constexpr (RES) pr[i] = ld_pack<T, V>(r + (int64_t)v * V);
+      px[i] = ld_once<T, V>(x + (int64_t)v * V);
+      if constexpr (RES) pr[i] = ld_once<T, V>(r + (int64_t)v * V);
     }
 #pragma unroll
     for (int i = 0; i < MAXV; ++i) {
@@ -304,7 +343,7 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlocksMin<V, MAXV>)
 #pragma unroll
       for (int j = 0; j < V; ++j) o.v[j] = divided_code<Q>(f.v[j], rstd, s);
     }
-    st_pack<uint8_t, V>(q + (int64_t)v * V, o);
+    st_once<uint8_t, V>(q + (int64_t)v * V, o);
   };
 
   if constexpr (MODE == kGroupLanes) {
