@@ -58,6 +58,50 @@ def test_w8a8_bias_act_refusals(fp8):
             op(*args, **kw)
 
 
+def test_overlaps_are_refused():
+    """An output over an operand, or part of the residual, would be read after it is written. What
+    is allowed goes on to the next check, that the tensors are on a GPU."""
+    buf, w, wide = Z(9, 4), Z(4, 4), Z(8, 12)
+    x, r = buf[:8], Z(8, 4)
+
+    def gemm(a, out, residual=None, bias=None, b=w):
+        return tob.gemm_bias_act(a, b, bias, residual=residual, out=out)
+
+    for args in [(x, x), (x, buf[1:])]:
+        with pytest.raises(ValueError, match="overlaps an input"):
+            gemm(*args)
+    with pytest.raises(ValueError, match="overlaps an input"):
+        gemm(Z(4, 4), w)
+    with pytest.raises(ValueError, match="overlaps an input"):
+        gemm(r, x, bias=buf[3])
+    with pytest.raises(ValueError, match="partly overlaps"):
+        gemm(r, x, residual=buf[1:])
+    with pytest.raises(ValueError, match="partly overlaps"):
+        gemm(Z(4, 4), x[:4], residual=x[:4].t())
+    with pytest.raises(ValueError, match="partly overlaps"):
+        gemm(r, wide[:, 2:6], residual=wide[:, :4])
+    for args in [(r, x, x), (r, x, buf[:8]), (wide[:, :4], wide[:, 4:8], wide[:, 8:]), (r, x, Z(8, 4))]:
+        with pytest.raises(TypeError, match="CUDA"):
+            gemm(*args)
+    a8 = Z(8, 8, dtype=torch.int8)
+    out = a8.view(torch.float16)  # [8, 4] over the operand's memory
+    with pytest.raises(ValueError, match="overlaps an input"):
+        tob.w8a8_block_int8_matmul_bias_act(a8, Z(4, 8, dtype=torch.int8), Z(8, 1), Z(4, 1), [1, 8],
+                                            out=out)
+
+    def norm(x, r, out, w=Z(4)):
+        return tob.add_rms_norm_group_quant(x, w, 4, r, residual_out=out)
+
+    for args in [(x, r, buf[1:]), (r, x, buf[1:])]:
+        with pytest.raises(ValueError, match="partly overlaps"):
+            norm(*args)
+    with pytest.raises(ValueError, match="overlaps an input"):
+        norm(r, Z(8, 4), x, buf[2])
+    for args in [(x, r, x), (x, r, r), (x, x, x), (wide[:, :4], wide[:, 4:8], wide[:, 8:])]:
+        with pytest.raises(TypeError, match="CUDA"):
+            norm(*args)
+
+
 def test_fnuz_operands_are_refused():
     a = Z(2, 8).to(torch.float8_e4m3fnuz)
     with pytest.raises(NotImplementedError, match="e4m3fn"):

@@ -10,7 +10,7 @@ from typing import Optional
 
 import torch
 
-from .fused import _row_stride
+from .fused import _refuse_overlap, _row_stride
 
 ACT_CODES = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
@@ -23,9 +23,10 @@ def _refuse(op: str, name: str, t: torch.Tensor, dtype: torch.dtype, device: tor
 
 def check(op: str, shape: tuple, n: int, dtype: torch.dtype, device: torch.device,
           bias: Optional[torch.Tensor], act: Optional[str], residual: Optional[torch.Tensor],
-          out: Optional[torch.Tensor]) -> int:
+          out: Optional[torch.Tensor], reads: tuple) -> int:
     """Checks the epilogue's operands against an output of ``shape`` (last dimension ``n``) and
-    returns the activation's code. Raised before any device work."""
+    returns the activation's code; ``reads``: the product's operands, which ``out`` must not
+    overlap. Raised before any device work."""
     try:
         code = ACT_CODES[act]
     except (KeyError, TypeError):
@@ -44,6 +45,8 @@ def check(op: str, shape: tuple, n: int, dtype: torch.dtype, device: torch.devic
         _refuse(op, "residual", residual, dtype, device)
     if out is not None and (out.dtype != dtype or out.device != device):
         _refuse(op, "out", out, dtype, device)
+    if out is not None:
+        _refuse_overlap(op, "out", out, (residual,), (*reads, bias))
     return code
 
 

@@ -62,7 +62,7 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
     bfloat16); ``act`` None, ``"relu"``, ``"silu"`` or ``"gelu"`` (tanh form, as in gelu_and_mul).
     The sum, the bias, the activation and the residual are fp32 and C is rounded once. Rows of A,
     residual and out may be strided. ``out`` may be ``residual`` (added in place); it must not
-    overlap A or B."""
+    overlap it otherwise, nor A, B or bias (ValueError)."""
     op = "gemm_bias_act"
     if a.ndim != 2 or b.ndim != 2:
         raise ValueError(f"{op} expects 2-D A and B")
@@ -77,7 +77,8 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
         raise ValueError(f"Unsupported dtype {dtype}; expected one of torch.float32, "
                          "torch.float16, torch.bfloat16")
     device = a.device
-    code = _epilogue.check(op, (m, n), n, dtype, device, bias, act, residual, out)
+    code = _epilogue.check(op, (m, n), n, dtype, device, bias, act, residual, out,
+                           (a, b))
     idx = _lib.ensure_device(a, op)
     if b.device != device:
         _lib.same_device(op, a, b)

@@ -157,6 +157,40 @@ def _refuse(op: str, name: str, t: torch.Tensor, dtype: torch.dtype,
     raise TypeError(f"{op}: all tensors must be on {device} ({name} is on {t.device})")
 
 
+def _span(t: torch.Tensor) -> int:
+    """Bytes from the first element of ``t`` to the end of its last."""
+    if t.is_contiguous():
+        return t.numel() * t.element_size()
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors share memory; column slices of the same rows do not."""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa + _span(a) <= pb or pb + _span(b) <= pa:
+        return False
+    la, lb = _row_stride(a), _row_stride(b)
+    if la is not None and lb is not None and a.dim() > 1 and b.dim() > 1:
+        pitch = la * a.element_size()
+        if pitch == lb * b.element_size() and pitch > 0:
+            off = (pb - pa) % pitch
+            return (off < a.shape[-1] * a.element_size() or
+                    off + b.shape[-1] * b.element_size() > pitch)
+    return True
+
+
+def _refuse_overlap(op: str, name: str, out: torch.Tensor, same: tuple, others: tuple) -> None:
+    """An output may be one of ``same``, in its layout, and shares memory with nothing else the
+    kernel reads."""
+    for t in same:
+        if t is not None and t is not out and _overlap(out, t) and (
+                t.data_ptr() != out.data_ptr() or t.stride() != out.stride()):
+            raise ValueError(f"{op}: {name} partly overlaps an input it may only replace whole")
+    for t in others:
+        if t is not None and _overlap(out, t):
+            raise ValueError(f"{op}: {name} overlaps an input")
+
+
 def add_rms_norm_group_quant(x: torch.Tensor, weight: torch.Tensor, group_size: int,
                              residual: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
                              dtype: Optional[torch.dtype] = None, quant_eps: float = 1e-10,
@@ -216,6 +250,7 @@ def add_rms_norm_group_quant(x: torch.Tensor, weight: torch.Tensor, group_size: 
                              f"x.shape={tuple(x.shape)}")
         if residual_out.dtype != xd or residual_out.device != device:
             _refuse(op, "residual_out", residual_out, xd, device)
+        _refuse_overlap(op, "residual_out", residual_out, (x, residual), (weight,))
     idx = _lib.ensure_device(x, op)
     if xd not in _DTYPES:
         raise TypeError(f"{op}: unsupported dtype {xd} (float32, float16 and bfloat16 are "

@@ -238,7 +238,8 @@ def _run_w8a8_bias_act(entry, op, a, b, a_s, b_s, block_n, block_k, m, n, k, bia
         raise TypeError(f"{op}: output_dtype {output_dtype} (float32, float16, bfloat16)")
     shape = (*a.shape[:-1], n)
     device = a.device
-    code = _epilogue.check(op, shape, n, output_dtype, device, bias, act, residual, out)
+    code = _epilogue.check(op, shape, n, output_dtype, device, bias, act, residual, out,
+                           (a, b, a_s, b_s))
     idx = _lib.ensure_device(a, op)
     _lib.same_device(op, a, b, a_s, b_s)
     if a_s.dtype != torch.float32 or not a_s.is_contiguous():
