@@ -1,7 +1,8 @@
 // Copies of a product's operands with 16-byte aligned, zero-padded rows, for the tiles that read
 // them by TMA: what a K or N that is no multiple of 16 bytes (or a pointer off alignment) costs a
-// product of many tokens is one pass over the operand. Bound by HBM: each operand read and written
-// once. Both operands in one launch.
+// product is one pass over the operand. Bound by HBM: each operand read and written once. Both
+// operands in one launch. One token 4097 x 4099 bf16 takes 23 us with its copies, 100 tokens 8191 x
+// 8191 93; realigned in registers inside the product they took 32 and 166.
 #include <algorithm>
 
 #include "linear_epi.cuh"
