@@ -48,15 +48,22 @@ def _row_stride(t: torch.Tensor) -> Optional[int]:
     cols = t.shape[-1]
     if cols > 1 and t.stride(-1) != 1:
         return None
-    if t.dim() == 1:
+    if t.numel() == 0:
         return cols
-    # the leading dimensions must collapse into one row index
-    for i in range(t.dim() - 2):
-        if t.shape[i] > 1 and t.stride(i) != t.stride(i + 1) * t.shape[i + 1]:
+    # The leading dimensions must collapse into one row index. Those of size 1 have no say: the
+    # pitch of [4, 1, 128][..., :64] is 128.
+    ld = outer = None
+    for i in range(t.dim() - 2, -1, -1):
+        n, step = t.shape[i], t.stride(i)
+        if n == 1:
+            continue
+        if ld is None:
+            ld = step
+        elif step != outer:
             return None
-    if t.shape[-2] <= 1:
+        outer = step * n
+    if ld is None:  # one row
         return cols
-    ld = t.stride(-2)
     return ld if ld >= cols else None
 
 
