@@ -1,0 +1,80 @@
+"""Order of the stream with programmatic dependent launches. A kernel that lets its successor start
+before its own predecessor has completed puts three kernels in flight, and with launch overlap on
+the third may read weights that the first still writes; set_launch_overlap promises that only the
+launch immediately before a call matters."""
+
+from __future__ import annotations
+
+import re
+from pathlib import Path
+
+import pytest
+import torch
+
+import tileops_b200 as tob
+
+CSRC = Path(tob.__file__).resolve().parent / "csrc"
+F64 = torch.float64
+
+
+def code(path):
+    return re.sub(r"//[^\n]*", "", path.read_text())
+
+
+@pytest.mark.parametrize("path", sorted(p for p in CSRC.glob("*.cu")
+                                        if "grid_dependents_launch()" in p.read_text()),
+                         ids=lambda p: p.name)
+def test_successors_start_after_the_wait(path):
+    """In every kernel, the wait for the previous kernel stands before the successor's start."""
+    for body in code(path).split("__global__")[1:]:
+        start = body.find("grid_dependents_launch()")
+        if start >= 0:
+            assert 0 <= body.find("grid_dependency_wait()") < start
+
+
+def ints(gen, lo, hi, *shape):
+    return torch.randint(lo, hi + 1, shape, generator=gen)
+
+
+@pytest.fixture
+def overlap():
+    prev = tob.set_launch_overlap(True)
+    yield
+    tob.set_launch_overlap(prev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("between", ["norm", "copies", "few_tokens", "pairs", "block_scaled"])
+@pytest.mark.parametrize("reader", ["gemv", "product"])
+def test_weights_written_two_launches_back(cuda, overlap, between, reader):
+    """An update of w, one operator, then a product that reads w. Whole numbers: every sum is exact
+    in fp32, so the result is that of the updated w, rounded once."""
+    gen = torch.Generator().manual_seed(1)
+    n = 4096
+    w0 = ints(gen, -2, 2, n, n).half().to(cuda)
+    la, lb = ints(gen, -1, 1, n, 16).half().to(cuda), ints(gen, -1, 1, 16, n).half().to(cuda)
+    x = ints(gen, -1, 1, 1, n).half().to(cuda)
+    m, k = {"norm": (8, 512), "copies": (4, 333), "few_tokens": (4, 512), "pairs": (2048, 64),
+            "block_scaled": (2048, 256)}[between]
+    y = ints(gen, -1, 1, m, k).half().to(cuda)
+    v = ints(gen, -1, 1, k, 2048).half().to(cuda)
+    y8, v8 = y.to(torch.int8), v.t().contiguous().to(torch.int8)
+    y_s, v_s = torch.ones(m, -(-k // 128), device=cuda), torch.ones(16, -(-k // 128), device=cuda)
+    ones = torch.ones(k, device=cuda).half()
+
+    def step():
+        if between == "norm":
+            tob.add_rms_norm_group_quant(y, ones, 128)
+        elif between == "block_scaled":
+            tob.w8a8_block_int8_matmul_bias_act(y8, v8, y_s, v_s, [128, 128])
+        else:
+            tob.gemm_bias_act(y, v)
+
+    w64 = w0.to(F64) + la.to(F64) @ lb.to(F64)
+    want = (w64 @ x[0].to(F64) if reader == "gemv" else x.to(F64) @ w64).half()
+    for _ in range(10):
+        w = w0.clone()
+        tob.gemm_bias_act(la, lb, residual=w, out=w)
+        step()
+        got = tob.gemv(w, x[0]) if reader == "gemv" else tob.gemm_bias_act(x, w)
+        assert torch.equal(got, want)

@@ -142,8 +142,6 @@ __global__ void __launch_bounds__(kThreadsB, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
 
-  if (threadIdx.x == 0) grid_dependents_launch();  // the next kernel may set itself up
-
   if (warp < kEpi0B) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (misaligned) {
@@ -154,6 +152,7 @@ __global__ void __launch_bounds__(kThreadsB, 1)
         const bool is_a = warp == 0;
         const uint64_t pol = policy_evict_normal();
         if (is_a || !ep.early_weights) grid_dependency_wait();
+        if (is_a) grid_dependents_launch();  // the next kernel may set itself up
         uint32_t issued_mask = 0, issued_phase = 0;
         bool ok = true;
         int it = 0;

@@ -51,7 +51,11 @@ __device__ __forceinline__ float act_gated(float x, const ActForm& f) {
 // every thread that touches global memory first waits for that kernel's completion
 // (griddepcontrol.wait), so the order of the stream holds as with plain launches. Only with launch
 // overlap switched on (to_set_launch_overlap) do the weights' copies skip that wait. Each block
-// waits before it ends, so completion stays transitive along a chain.
+// waits before it ends, so completion stays transitive along a chain. A block lets the next kernel
+// start (griddepcontrol.launch_dependents) only after its own wait: at most two kernels of a stream
+// are in flight, so a later kernel that reads its weights early (launch overlap) can meet its
+// immediate predecessor alone, never a writer further back. (The later start costs 0.1 to 0.2 us a
+// launch: the norm of one token 2.1 us before, 2.2 so.)
 
 // What a product's epilogue reads and writes besides the accumulators. Row strides in elements.
 struct LinEpi {

@@ -125,7 +125,6 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS>::kThreads,
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   bool ok = !misaligned;
-  if (threadIdx.x == 0) grid_dependents_launch();  // the next kernel may set itself up
   if (S > 1) cluster_arrive_relaxed();  // this CTA runs: its shared memory may be stored to
 
   if (!ok) {
@@ -137,6 +136,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS>::kThreads,
       // The weights stream once past L2's other contents; every column tile re-reads the tokens.
       const uint64_t pol = wts ? policy_evict_first() : policy_evict_last();
       if (!wts || !g.ep.early_weights) grid_dependency_wait();
+      if (!wts) grid_dependents_launch();  // the next kernel may set itself up
       uint32_t issued_mask = 0, issued_phase = 0;
       for (int it = 0; it < kb_n; ++it) {
         const int s = it % ST;

@@ -125,8 +125,6 @@ __global__ void __launch_bounds__(kThreadsP, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
 
-  if (threadIdx.x == 0) grid_dependents_launch();  // the next kernel may set itself up
-
   if (misaligned) {
     // nothing to do; fall through to the teardown
   } else if (warp == 0 || warp == kBWarpP) {
@@ -138,6 +136,7 @@ __global__ void __launch_bounds__(kThreadsP, 1)
                                       : policy_evict_first();
       const uint32_t lead_full = mapa_shared(smem_u32(full), 0);
       if (is_a || !ep.early_weights) grid_dependency_wait();
+      if (is_a) grid_dependents_launch();  // the next kernel may set itself up
       uint32_t issued_mask = 0, issued_phase = 0;
       bool ok = true;
       int it = 0;  // stages issued

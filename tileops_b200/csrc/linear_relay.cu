@@ -21,8 +21,8 @@ constexpr int kRelayThreads = 256, kRelayBatch = 4;
 
 __global__ void __launch_bounds__(kRelayThreads)
     k_linear_relay(const RelayJob j0, const RelayJob j1, int blocks0) {
-  grid_dependents_launch();
   grid_dependency_wait();  // a programmatic dependent, as the products are
+  grid_dependents_launch();
   const bool first = (int)blockIdx.x < blocks0;
   const RelayJob j = first ? j0 : j1;
   const int64_t blocks = first ? blocks0 : (int64_t)gridDim.x - blocks0;

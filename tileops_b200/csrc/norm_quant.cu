@@ -209,9 +209,9 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlocksMin<V, MAXV>)
   __shared__ float red[2][32];
   extern __shared__ unsigned gmax[];  // kGroupShared: [rows of the CTA][groups]
   // Launched as a programmatic dependent: blocks may start while the previous kernel drains, and
-  // wait for its completion before they touch memory.
-  grid_dependents_launch();
+  // wait for its completion before they touch memory or let the next kernel start.
   grid_dependency_wait();
+  grid_dependents_launch();
   const int team = a.team;
   int tid = (int)threadIdx.x, local = 0;
   if (team < (int)blockDim.x) {
