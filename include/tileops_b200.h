@@ -85,7 +85,8 @@ TO_API int to_wait_limit_selftest(int limit_us, int arrive, unsigned long long* 
  * completed. Use it for chains of layers whose weights no kernel in the stream writes (a
  * decode loop); leave it off (the default) when a kernel that writes the weights, such as
  * to_awq_pack, may be the immediately preceding launch. enable < 0 only queries. Returns the
- * previous setting. Process-wide. No reference counterpart (a launch-policy extension). */
+ * previous setting. Process-wide. The *_bias_act products and to_add_rms_norm_group_quant read
+ * nothing ahead whatever it says. No reference counterpart (a launch-policy extension). */
 TO_API int to_set_launch_overlap(int enable);
 
 /* ---- symmetric INT8 (tileops/quant.py) ------------------------------------------------

@@ -78,3 +78,48 @@ def test_weights_written_two_launches_back(cuda, overlap, between, reader):
         step()
         got = tob.gemv(w, x[0]) if reader == "gemv" else tob.gemm_bias_act(x, w)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("path", sorted(CSRC.glob("linear_*")) + [CSRC / "norm_quant.cu"],
+                         ids=lambda p: p.name)
+def test_products_with_an_epilogue_read_nothing_ahead(path):
+    """No wait of these kernels is conditional on the launch-overlap switch."""
+    text = code(path)
+    assert "launch_overlap" not in text and "early_weights" not in text
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 4096), (40, 2048, 1000), (1000, 1024, 2048),
+                                   (4, 1001, 3001)])
+def test_weights_written_by_the_launch_before(cuda, overlap, m, k, n):
+    """A weight handed over transposed (the call copies it first), or written by the launch just
+    before the call, through the few-token and pair tiles and the aligned copies."""
+    gen = torch.Generator().manual_seed(m)
+    a = ints(gen, -2, 2, m, k).half().to(cuda)
+    wt = ints(gen, -2, 2, n, k).half().to(cuda)
+    want = (a.to(F64) @ wt.to(F64).t()).half()
+    want2 = (a.to(F64) @ (wt.to(F64) + 1).t()).half()
+    for _ in range(10):
+        assert torch.equal(tob.gemm_bias_act(a, wt.t()), want)
+        w = wt.t().contiguous()
+        w.add_(1)
+        assert torch.equal(tob.gemm_bias_act(a, w), want2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("codes", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("block", [[1, 4096], [128, 128]])
+@pytest.mark.parametrize("m", [1, 40, 600])
+def test_codes_written_by_the_launch_before(cuda, overlap, codes, block, m):
+    gen = torch.Generator().manual_seed(m)
+    k, n = 4096, 1536
+    a, w = ints(gen, -2, 2, m, k).to(codes).to(cuda), ints(gen, -3, 3, n, k).to(codes).to(cuda)
+    a_s = torch.ones(m, -(-k // block[1]), device=cuda)
+    b_s = torch.ones(-(-n // block[0]), -(-k // block[1]), device=cuda)
+    op = (tob.w8a8_block_int8_matmul_bias_act if codes == torch.int8
+          else tob.w8a8_block_fp8_matmul_bias_act)
+    want = (a.to(torch.float32).to(F64) @ w.to(torch.float32).to(F64).t()).float()
+    for _ in range(10):
+        v = torch.zeros_like(w)
+        v.copy_(w)
+        assert torch.equal(op(a, v, a_s, b_s, block, output_dtype=torch.float32), want)

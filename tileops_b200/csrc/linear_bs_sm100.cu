@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kThreadsB, 1)
       if (lane == 0) {
         const bool is_a = warp == 0;
         const uint64_t pol = policy_evict_normal();
-        if (is_a || !ep.early_weights) grid_dependency_wait();
+        grid_dependency_wait();
         if (is_a) grid_dependents_launch();  // the next kernel may set itself up
         uint32_t issued_mask = 0, issued_phase = 0;
         bool ok = true;

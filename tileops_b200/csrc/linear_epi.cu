@@ -26,8 +26,8 @@ LinOps make_ops(const void* a, int64_t lda, const void* b, int64_t M, int64_t N,
 
 // Many tokens: CTA-pair tiles, or folding tiles with block scales; few tokens or a small grid: weights
 // as rows. All of them over aligned copies of the operands that TMA cannot read.
-int tensor_core_launch(const char* op, int kind, bool block_scaled, LinOps o, LinEpi ep, void* ws,
-                       size_t ws_bytes, cudaStream_t st) {
+int tensor_core_launch(const char* op, int kind, bool block_scaled, LinOps o, const LinEpi& ep,
+                       void* ws, size_t ws_bytes, cudaStream_t st) {
   const int64_t need = linear_relay_bytes(kind, o);
   if (need > 0) {
     if (!ws || (int64_t)ws_bytes < need)
@@ -36,7 +36,6 @@ int tensor_core_launch(const char* op, int kind, bool block_scaled, LinOps o, Li
     if (!aligned16(ws)) return fail(TO_EINVAL, "%s: workspace is not 16-byte aligned", op);
     const int rc = linear_relay(kind, &o, ws, st);
     if (rc) return rc;
-    ep.early_weights = 0;  // the copies are the previous kernel's output
   }
   const int rc = block_scaled ? sm100::linear_bs_launch(kind, o, ep, st)
                               : sm100::linear_pair_launch(kind, o, ep, st);
@@ -64,7 +63,6 @@ int make_epi(LinEpi* ep, const char* op, const void* bias, int act, const void* 
   ep->dtype = dtype;
   ep->act = act;
   ep->form = act_form(act);
-  ep->early_weights = launch_overlap();
   return TO_OK;
 }
 

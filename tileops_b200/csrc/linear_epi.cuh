@@ -49,9 +49,11 @@ __device__ __forceinline__ float act_gated(float x, const ActForm& f) {
 // Launches of these kernels carry the programmatic-dependency attribute always: a kernel's blocks may
 // start (barriers, tensor memory, tensor maps) while the previous kernel of the stream drains, and
 // every thread that touches global memory first waits for that kernel's completion
-// (griddepcontrol.wait), so the order of the stream holds as with plain launches. Only with launch
-// overlap switched on (to_set_launch_overlap) do the weights' copies skip that wait. Each block
-// waits before it ends, so completion stays transitive along a chain. A block lets the next kernel
+// (griddepcontrol.wait), so the order of the stream holds as with plain launches, whatever the
+// launch-overlap switch says: the weights' copies wait too, since a B that the caller hands over
+// in another layout has just been copied. (Weights read ahead with overlap on saved 0.4 to 0.7 us
+// a call: 4096 x 4096, one token, 8.0 against 8.5.) Each block waits before it ends, so completion
+// stays transitive along a chain. A block lets the next kernel
 // start (griddepcontrol.launch_dependents) only after its own wait: at most two kernels of a stream
 // are in flight, so a later kernel that reads its weights early (launch overlap) can meet its
 // immediate predecessor alone, never a writer further back. (The later start costs 0.1 to 0.2 us a
@@ -70,7 +72,6 @@ struct LinEpi {
   int64_t ldr = 0, ldc = 0;
   int dtype = TO_F32;
   int act = kActNone;
-  int early_weights = 0;       // launch overlap: weights are read before the previous kernel ends
   ActForm form = {};           // act_form(act)
 };
 

@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS>::kThreads,
       const bool wts = warp == 0;
       // The weights stream once past L2's other contents; every column tile re-reads the tokens.
       const uint64_t pol = wts ? policy_evict_first() : policy_evict_last();
-      if (!wts || !g.ep.early_weights) grid_dependency_wait();
+      grid_dependency_wait();
       if (!wts) grid_dependents_launch();  // the next kernel may set itself up
       uint32_t issued_mask = 0, issued_phase = 0;
       for (int it = 0; it < kb_n; ++it) {

@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kThreadsP, 1)
                            : is_a     ? policy_evict_last()
                                       : policy_evict_first();
       const uint32_t lead_full = mapa_shared(smem_u32(full), 0);
-      if (is_a || !ep.early_weights) grid_dependency_wait();
+      grid_dependency_wait();
       if (is_a) grid_dependents_launch();  // the next kernel may set itself up
       uint32_t issued_mask = 0, issued_phase = 0;
       bool ok = true;
