@@ -88,6 +88,20 @@ def test_products_with_an_epilogue_read_nothing_ahead(path):
     assert "launch_overlap" not in text and "early_weights" not in text
 
 
+@pytest.mark.parametrize("name", ["linear_nt_sm100.cu", "linear_pair_sm100.cu",
+                                  "linear_bs_sm100.cu"])
+def test_bounded_waits_start_after_the_previous_kernel(name):
+    """Every role of a product's blocks waits for the previous kernel before its first bounded wait,
+    so that a predecessor which runs longer than the limit does not use it up."""
+    body = (CSRC / name).read_text().split("__global__")[1]
+    waits = ("mbar_wait_polled(", "mbar_wait_warp(", "mbar_wait(")
+    roles = [re.sub(r"//[^\n]*", "", r) for r in re.split(r"// -{20,}", body)[1:]]
+    roles = [r for r in roles if any(w in r for w in waits)]
+    assert len(roles) >= 3
+    for r in roles:
+        assert 0 <= r.find("grid_dependency_wait()") < min(r.find(w) for w in waits if w in r)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,k,n", [(1, 4096, 4096), (40, 2048, 1000), (1000, 1024, 2048),
                                    (4, 1001, 3001)])

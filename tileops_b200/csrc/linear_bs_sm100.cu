@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(kThreadsB, 1)
       const uint64_t adesc = smem_desc_kmajor_sw128(smem_u32(sA));
       const uint64_t bdesc = smem_desc_kmajor_sw128(smem_u32(sB));
       const bool issue = elect_one();
+      grid_dependency_wait();  // the waits below count this kernel's time, not the previous one's
       bool ok = true;
       int it = 0, s = 0;
       uint32_t ph = 0;

@@ -179,6 +179,7 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS>::kThreads,
                                   : smem_desc_kmajor_sw128(smem_u32(sW));
     const uint64_t xdesc = smem_desc_kmajor_sw128(smem_u32(sX));
     const bool issue = elect_one();
+    grid_dependency_wait();  // the waits below count this kernel's time, not the previous one's
     bool any = false;
     int s = 0;
     uint32_t ph = 0;

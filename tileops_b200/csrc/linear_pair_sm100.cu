@@ -213,6 +213,7 @@ __global__ void __launch_bounds__(kThreadsP, 1)
       const uint64_t bdesc = C::kMn ? smem_desc_mnmajor_sw128(smem_u32(sB), 16384, 1024)
                                     : smem_desc_kmajor_sw128(smem_u32(sB));
       const bool issue = elect_one();
+      grid_dependency_wait();  // the waits below count this kernel's time, not the previous one's
       bool ok = true;
       int fill = 0, s = 0;  // accumulator fills started; stage
       uint32_t ph = 0;
