@@ -320,7 +320,9 @@ TO_API size_t to_w8a8_gemm_bias_act_workspace_size(const void* a, const void* b,
  * a_s[m,kb] b_s[n/block_n,kb] + bias) + residual. Operands and scales as to_w8a8_i8_gemm /
  * to_w8a8_fp8_gemm; bias, residual and C of c_dtype. One rounding (to_w8a8_*_gemm with a bias
  * rounds twice, as the reference does). block_k >= K or a multiple of 128 runs on tcgen05 tiles,
- * any other block_k on SIMT tiles. */
+ * any other block_k on SIMT tiles. int8: a block's sum is an exact int32; one block of K > 131071,
+ * which that cannot hold, is summed in fp32 over exact sums of 128 products, and a block_k > 131071
+ * on the SIMT tiles is refused (TO_EUNSUPPORTED). */
 TO_API int to_w8a8_i8_gemm_bias_act(const int8_t* a, const int8_t* b, const float* a_s,
                                     const float* b_s, const void* bias, int act,
                                     const void* residual, int64_t ldr, void* c, int64_t ldc,

@@ -19,6 +19,9 @@ int linear_w8a8_simt_launch(bool fp8, const void* a, const void* b, int64_t M, i
 
 namespace {
 
+// Products of int8 codes that an int32 sum holds whatever they are: (-128)^2 x 131072 is 2^31.
+constexpr int64_t kInt32Terms = 131071;
+
 LinOps make_ops(const void* a, int64_t lda, const void* b, int64_t M, int64_t N, int64_t K,
                 bool b_mn) {
   return LinOps{a, b, lda, b_mn ? N : K, K, b_mn ? N : K, M, N, K};
@@ -87,10 +90,17 @@ int w8a8_epi_entry(bool fp8, const void* a, const void* b, const float* a_s, con
   ep.bn = bn >= N ? N : bn;
   cudaStream_t st = (cudaStream_t)stream;
   // The tensor-core tiles change scales on whole 128-byte K slices; one K block needs none.
-  if (kt > 1 && bk % 128 != 0)
+  if (kt > 1 && bk % 128 != 0) {
+    if (!fp8 && bk > kInt32Terms)
+      return fail(TO_EUNSUPPORTED, "%s: block_k=%lld, an int32 block sum holds %lld products (or a "
+                  "multiple of 128)", op, (long long)bk, (long long)kInt32Terms);
     return linear_w8a8_simt_launch(fp8, a, b, M, N, K, ep.bn, bk, ep, st);
-  ep.kb_per_scale = kt > 1 ? (int)(bk / 128) : 1;
-  return tensor_core_launch(op, fp8 ? TO_E4M3 : TO_I8, kt > 1, make_ops(a, K, b, M, N, K, false), ep,
+  }
+  // One block of more products than int32 holds: its 128-product slices are added up in fp32, as if
+  // each were a block of its own with the same scales.
+  const bool fold = kt > 1 || (!fp8 && K > kInt32Terms);
+  ep.kb_per_scale = (int)(kt > 1 ? bk / 128 : ceil_div(K, 128));
+  return tensor_core_launch(op, fp8 ? TO_E4M3 : TO_I8, fold, make_ops(a, K, b, M, N, K, false), ep,
                             ws, ws_bytes, st);
 }
 
