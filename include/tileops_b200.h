@@ -299,8 +299,9 @@ TO_API int to_gemm(const void* a, const void* b, void* c, int dtype, int64_t M, 
 /* Library extension (no reference counterpart): C = act(A @ B + bias) + residual in one kernel;
  * A [M,K] rows lda apart, B [K,N] dense, bias [N] or NULL, residual [M,N] rows ldr apart or NULL,
  * C [M,N] rows ldc apart, all of dtype F32, F16 or BF16; act one of TO_EPI_*. fp32 up to the one
- * rounding of C. C may be the residual; it must not overlap A or B. Any M, N, K (K = 0: the
- * epilogue of zeros). 16-bit operands run on tcgen05 tiles at any alignment, fp32 on SIMT tiles.
+ * rounding of C. C may be the residual; it must not overlap A or B. M, N and K up to
+ * 2^31 - 1024 (K = 0: the epilogue of zeros), M up to 65535 x 64 on the SIMT tiles; more is refused.
+ * 16-bit operands run on tcgen05 tiles at any alignment, fp32 and K = 0 on SIMT tiles.
  * workspace as to_gemm_bias_act_workspace_size says. */
 #define TO_EPI_NONE 0
 #define TO_EPI_RELU 1
@@ -322,7 +323,8 @@ TO_API size_t to_w8a8_gemm_bias_act_workspace_size(const void* a, const void* b,
  * rounds twice, as the reference does). block_k >= K or a multiple of 128 runs on tcgen05 tiles,
  * any other block_k on SIMT tiles. int8: a block's sum is an exact int32; one block of K > 131071,
  * which that cannot hold, is summed in fp32 over exact sums of 128 products, and a block_k > 131071
- * on the SIMT tiles is refused (TO_EUNSUPPORTED). */
+ * on the SIMT tiles is refused (TO_EUNSUPPORTED). Dimensions as above; block scales whose block_n is
+ * no multiple of 32 take at most 65535 x 64 rows, too. */
 TO_API int to_w8a8_i8_gemm_bias_act(const int8_t* a, const int8_t* b, const float* a_s,
                                     const float* b_s, const void* bias, int act,
                                     const void* residual, int64_t ldr, void* c, int64_t ldc,
@@ -368,7 +370,9 @@ TO_API int to_act_and_mul_group_quant(const void* a, const void* b, int dtype, i
 /* Library extension (no reference counterpart): residual add, root-mean-square norm and per-group
  * quantisation of [rows, cols] in one pass: h = x + residual (residual may be NULL), y = h /
  * sqrt(mean(h^2) + eps) * weight, scale = max(max|y|, quant_eps) / qmax per group of group_size
- * columns (group_size divides cols; eps >= 0, quant_eps >= 1e-35; q_dtype TO_E4M3: qmax 448, ue8m0 and column_major as
+ * columns (group_size divides cols; cols at most 2^31 - 1024, groups of a row at most 51200 unless
+ * group_size is all of cols or 1 to 32 packs of 16 bytes, a power of two of them, with 16-byte aligned
+ * rows; eps >= 0, quant_eps >= 1e-35; q_dtype TO_E4M3: qmax 448, ue8m0 and column_major as
  * to_per_token_group_quant_fp8; TO_I8: 127), q [rows, cols] the codes of y / scale, dense. fp32
  * throughout; y is not rounded to dtype. h rounded to dtype goes to residual_out, given exactly
  * when residual is (x or residual itself allowed). x, residual, residual_out rows ldx, ldr, ldh apart; weight

@@ -45,6 +45,10 @@ inline const char* tuning_env(const char* name) {
   return nullptr;
 #endif
 }
+// The largest dimension that the fused norm quantiser and the products with an epilogue take: their
+// kernels round indexes up to whole tiles and strides in 32 bits, and 1023 below 2^31 none of those
+// sums wraps (the widest step is 512).
+constexpr int64_t kDimMax = INT32_MAX - 1023;
 // Codes kernels write into the error word.
 enum DeviceError : int { kErrNone = 0, kErrWaitTimeout = 1, kErrTmemAlloc = 2, kErrSmemAlign = 3 };
 

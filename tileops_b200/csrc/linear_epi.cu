@@ -74,8 +74,8 @@ int w8a8_epi_entry(bool fp8, const void* a, const void* b, const float* a_s, con
                    int c_dtype, int64_t M, int64_t N, int64_t K, int64_t bn, int64_t bk,
                    void* ws, size_t ws_bytes, void* stream) {
   const char* op = fp8 ? "w8a8_block_fp8_matmul_bias_act" : "w8a8_block_int8_matmul_bias_act";
-  if (M < 0 || N < 0 || K <= 0 || bn <= 0 || bk <= 0 || M > INT32_MAX || N > INT32_MAX ||
-      K > INT32_MAX)
+  if (M < 0 || N < 0 || K <= 0 || bn <= 0 || bk <= 0 || M > kDimMax || N > kDimMax ||
+      K > kDimMax)
     return fail(TO_EINVAL, "%s: invalid M=%lld N=%lld K=%lld block=[%lld,%lld]", op, (long long)M,
                 (long long)N, (long long)K, (long long)bn, (long long)bk);
   LinEpi ep;
@@ -126,7 +126,7 @@ int to_gemm_bias_act(const void* a, int64_t lda, const void* b, const void* bias
                      int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace tob;
   const char* op = "gemm_bias_act";
-  if (M < 0 || N < 0 || K < 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX)
+  if (M < 0 || N < 0 || K < 0 || M > kDimMax || N > kDimMax || K > kDimMax)
     return fail(TO_EINVAL, "%s: invalid shape M=%lld N=%lld K=%lld", op, (long long)M,
                 (long long)N, (long long)K);
   if (M > 1 && lda < K)

@@ -538,7 +538,7 @@ extern "C" int to_add_rms_norm_group_quant(
     void* stream) {
   using namespace tob;
   const char* op = "add_rms_norm_group_quant";
-  if (rows < 0 || cols < 0 || cols > INT32_MAX || group_size <= 0 || cols % group_size != 0 ||
+  if (rows < 0 || cols < 0 || cols > kDimMax || group_size <= 0 || cols % group_size != 0 ||
       (rows > 1 && (ldx < cols || (residual && ldr < cols) || (residual_out && ldh < cols))))
     return fail(TO_EINVAL, "%s: invalid shape rows=%lld cols=%lld group=%lld strides=(%lld, %lld, "
                 "%lld)", op, (long long)rows, (long long)cols, (long long)group_size,
