@@ -46,6 +46,20 @@ __device__ __forceinline__ float act_gated(float x, const ActForm& f) {
   return __fdividef(x, 1.0f + e);
 }
 
+// The gated forms for fp32 results, of which that error would be many steps: the accurate
+// exponential, and the quotient by Markstein's correction (q + (x - q d) / d from an approximate
+// reciprocal of d), which has no branches as the division operator has: with that, the epilogue of
+// 8192 x 1024 -> 8192 made 180 us 490. Where the correction is no number (x or d infinite) the
+// first quotient stands: inf, 0 or NaN as x / d.
+__device__ __forceinline__ float act_gated_f32(float x, int act) {
+  const float z = act == kActSilu ? x : 1.5957691216057308f * fmaf(0.044715f * x * x, x, x);
+  const float d = 1.0f + expf(-z);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  const float q = x * r, t = fmaf(-q, d, x);
+  return t == t ? fmaf(t, r, q) : q;
+}
+
 // Launches of these kernels carry the programmatic-dependency attribute always: a kernel's blocks may
 // start (barriers, tensor memory, tensor maps) while the previous kernel of the stream drains, and
 // every thread that touches global memory first waits for that kernel's completion

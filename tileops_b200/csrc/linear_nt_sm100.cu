@@ -240,8 +240,10 @@ __global__ void __launch_bounds__(NtCfg<KD, NT, BS>::kThreads,
   // One output of token tok: acc is its scaled sum.
   auto finish = [&](float acc, int tok, float res) {
     const float v = acc + bias;
-    const float y = (ep.form.gated ? act_gated(v, ep.form) : act_plain(v, ep.form)) + res;
-    st_dtype(ep.c, (int64_t)(t0 + tok) * ep.ldc + n, ep.dtype, y);
+    const float y = !ep.form.gated       ? act_plain(v, ep.form)
+                    : ep.dtype == TO_F32 ? act_gated_f32(v, ep.act)
+                                         : act_gated(v, ep.form);
+    st_dtype(ep.c, (int64_t)(t0 + tok) * ep.ldc + n, ep.dtype, y + res);
   };
   if (S > 1) cluster_wait_acquire();  // so do the peers
   if (epi && ok) {

@@ -4,6 +4,8 @@
 
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "linear_epi.cuh"
 #include "sm100.cuh"
 
@@ -72,8 +74,9 @@ struct ChunkWriter {
     return true;
   }
   // v: this lane's row of the chunk, scaled; bias: of its 32 columns, in shared memory. Straight
-  // code per step, one uniform choice around each (see ActForm).
-  __device__ __forceinline__ void finish_acts(float* v, const float* bias) {
+  // code per step, one uniform choice around each (see ActForm). F32: the result is fp32.
+  template <bool F32 = false>
+  __device__ __forceinline__ void finish_acts(float* v, const float* bias, int act = kActNone) {
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
       const float4 b = *reinterpret_cast<const float4*>(bias + i);
@@ -82,7 +85,13 @@ struct ChunkWriter {
       v[i + 2] += b.z;
       v[i + 3] += b.w;
     }
-    if (form.gated) {
+    if (F32 && act == kActSilu) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = act_gated_f32(v[i], kActSilu);
+    } else if (F32 && act == kActGelu) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = act_gated_f32(v[i], kActGelu);
+    } else if (!F32 && form.gated) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = act_gated(v[i], form);
     } else {
@@ -105,7 +114,7 @@ struct ChunkWriter {
       for (int r = 0; r < 16; ++r, rp += ep.ldr) f[r] = *rp;
     };
     if (ep.res != nullptr && mine && whole) fetch_rows();
-    finish_acts(v, bias);
+    finish_acts<std::is_same<T, float>::value>(v, bias, ep.act);
     float* turn = reinterpret_cast<float*>(slab0);
     __syncwarp();  // the previous chunk has been read
 #pragma unroll
