@@ -99,3 +99,18 @@ def test_gated_activations_of_one_token_slices(cuda):
     q, s = tob.act_and_mul_group_quant(gate, up, 128)
     q0, s0 = tob.act_and_mul_group_quant(gate.contiguous(), up.contiguous(), 128)
     assert torch.equal(q.view(torch.uint8), q0.view(torch.uint8)) and torch.equal(s, s0)
+
+
+def test_in_place_through_another_view():
+    """One row of a wide buffer, as a slice and as an unsqueezed row: the strides of the size-1
+    dimension differ, the memory does not. What is allowed goes on to the check for a GPU."""
+    buf, w = Z(5, 16), Z(4, 4)
+    row, again = buf[:1, :4], buf[0, :4][None]
+    assert row.stride() != again.stride()
+    a = Z(1, 4)
+    with pytest.raises(TypeError, match="CUDA"):
+        tob.gemm_bias_act(a, w, residual=row, out=again)
+    with pytest.raises(TypeError, match="CUDA"):
+        tob.add_rms_norm_group_quant(a, Z(4), 4, row, residual_out=again)
+    with pytest.raises(ValueError, match="partly overlaps"):
+        tob.gemm_bias_act(a, w, residual=row, out=buf[:1, 1:5])

@@ -186,12 +186,17 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return True
 
 
+def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether element i of both is the same memory; a dimension of size 1 has any stride."""
+    return a.data_ptr() == b.data_ptr() and all(
+        n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
 def _refuse_overlap(op: str, name: str, out: torch.Tensor, same: tuple, others: tuple) -> None:
     """An output may be one of ``same``, in its layout, and shares memory with nothing else the
     kernel reads."""
     for t in same:
-        if t is not None and t is not out and _overlap(out, t) and (
-                t.data_ptr() != out.data_ptr() or t.stride() != out.stride()):
+        if t is not None and t is not out and _overlap(out, t) and not _same_layout(out, t):
             raise ValueError(f"{op}: {name} partly overlaps an input it may only replace whole")
     for t in others:
         if t is not None and _overlap(out, t):
