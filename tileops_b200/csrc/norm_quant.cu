@@ -7,7 +7,10 @@
 // rstd is one factor of a whole row, so what waits for the row's sum is one number: p = h w stays in
 // registers, max|y| = rstd max|p| per group, and a code is the code of p c with c = rstd / s.
 //
-// Bound by HBM: 2 + 2 B read, 2 + 1 B written per element (16-bit input); x and r are read once. A
+// Bound by HBM: 2 + 2 B read, 2 + 1 B written per element (16-bit input); x and r are read once by
+// rows that a block holds: 16-bit rows of up to 16384 columns where there are as many SMs as rows, of
+// 8192 up to two rows an SM, of 12288 beyond. What a longer row has left is read again, once or
+// (groups off the packs) twice, mostly from L2. A
 // team of threads (whole warps) holds a row, MAXV 16-byte packs per thread; the group maxima are
 // shuffles where a group is a power-of-two number of packs within a warp, the team's reduction
 // (with the sum's) where it is the row, and shared-memory maxima (order-independent) for any other
@@ -191,12 +194,16 @@ __device__ __noinline__ uint8_t divided_code(float p, float rstd, float s) {
 }
 
 // Threads of a block at most, and blocks of an SM the registers are sized for. 32 values a thread
-// (four 16-byte packs of 16-bit values) want 80 registers, 16 or fewer fit 64. Many rows run on
-// blocks of 512 threads at most, so that an SM always holds two and one's loads cover the other's
-// arithmetic (a row of 13248 columns on one block of 832 threads per SM took three times as long);
-// what a longer row has left is re-read.
-template <int V, int MAXV> constexpr int kBlockMax = V * MAXV > 16 ? 384 : V * MAXV == 16 ? 512 : 1024;
-template <int V, int MAXV> constexpr int kBlocksMin = V * MAXV >= 16 ? 2 : 1;
+// (four 16-byte packs of 16-bit values) want 80 registers, 16 or fewer fit 64 (16 single values do
+// not: that form spills some 100 to 500 bytes). Many rows run on blocks of 512 threads at most, so
+// that an SM always holds two and one's loads cover the other's arithmetic (a row of 13248 columns on
+// one block of 832 threads per SM took three times as long); what a longer row has left is re-read.
+// Two packs of 16-bit values serve few rows alone, see block_threads.
+template <int V, int MAXV> constexpr bool kFewRows = V == 8 && MAXV == 2;
+template <int V, int MAXV>
+constexpr int kBlockMax = V * MAXV > 16 ? 384 : V * MAXV == 16 && !kFewRows<V, MAXV> ? 512 : 1024;
+template <int V, int MAXV>
+constexpr int kBlocksMin = V * MAXV >= 16 && !kFewRows<V, MAXV> ? 2 : 1;
 
 // One block per rows_per_block rows, a team of threads each. RES: with a residual and its output.
 // Loads are not guarded but clamped (rows and packs past the end re-read the last and count as
@@ -444,13 +451,23 @@ __global__ void __launch_bounds__(kBlockMax<V, MAXV>, kBlocksMin<V, MAXV>)
   }
 }
 
+// Threads a block has at most. Two packs a thread: 1024 threads hold a row of 2048 packs where every
+// row has an SM to itself; with more rows two blocks of 512 on an SM are faster although they read
+// the rest of a row again. fp16, G = row, 16384 columns: 64 rows 3.83 us on 512 threads, 3.44 on 1024;
+// 256 rows 6.65 and 8.19 (11008 columns: 3.22, 2.92; 5.02, 6.45). Four packs on 384 threads: 4.27 and
+// 6.75 (3.26, 4.91).
+template <int V, int MAXV>
+int block_threads(int64_t rows) {
+  return kFewRows<V, MAXV> && rows > sm_count() ? 512 : kBlockMax<V, MAXV>;
+}
+
 template <typename T, int Q, int V, int MAXV, int MODE>
 int launch_norm(NormArgs a, cudaStream_t st) {
   auto kern = a.h != nullptr ? k_norm_quant<T, Q, V, MAXV, MODE, true>
                              : k_norm_quant<T, Q, V, MAXV, MODE, false>;
   const int64_t nvec = a.cols / V;
   int64_t team = ceil_div(ceil_div(nvec, MAXV), 32) * 32;
-  if (team > kBlockMax<V, MAXV>) team = kBlockMax<V, MAXV>;
+  team = std::min<int64_t>(team, block_threads<V, MAXV>(a.rows));
   a.team = (int)team;
   // Small rows share a CTA of up to 256 threads.
   int64_t per_cta = std::max<int64_t>(1, 256 / team);
@@ -514,8 +531,8 @@ int launch_norm_any(const NormArgs& a, cudaStream_t st) {
                    : a.G == a.cols                          ? kGroupRow
                                                             : kGroupShared;
   if (mode == kGroupShared) return launch_norm<T, Q, VV, 4, kGroupShared>(a, st);
-  // Packs per thread: few rows (two per SM) take as few as keep a row in one block, for latency;
-  // many take four, for bytes in flight at few threads.
+  // Packs per thread: few rows (two per SM) take one where a block holds the row so and two up to
+  // 2048 packs, for latency; many, and longer rows, take four, for bytes in flight at few threads.
   const int64_t nvec = a.cols / VV;
   const int maxv = a.rows > 2 * sm_count() || nvec > 2048 ? 4 : nvec <= 1024 ? 1 : 2;
   auto run = [&](auto m) {
