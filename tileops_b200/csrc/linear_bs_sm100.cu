@@ -442,7 +442,7 @@ static int bs_width(int64_t M, int64_t N, int64_t bn) {
 int linear_bs_launch(int kind, const LinOps& o, const LinEpi& ep, cudaStream_t st) {
   const int best = bs_width(o.M, o.N, ep.bn);
   if (best == 0 || !aligned_rows(o.a, o.lda) || !aligned_rows(o.b, o.ldb)) return TO_EUNSUPPORTED;
-  const bool plain = plain_output(ep);
+  const bool plain = plain_output(ep, o.N);
   auto run = [&](auto kd) {
     constexpr Kind KD = decltype(kd)::value;
     switch (best) {

@@ -462,7 +462,7 @@ int linear_pair_launch(int kind, const LinOps& o, const LinEpi& ep, cudaStream_t
   const int best = pair_width(kind, o.M, o.N);
   if (best == 0 || !aligned_rows(o.a, o.lda * e) || !aligned_rows(o.b, o.ldb * e))
     return TO_EUNSUPPORTED;
-  const bool plain = plain_output(ep);
+  const bool plain = plain_output(ep, o.N);
   if (kind == TO_F16)
     return best == 256 ? launch_pair<Kind::F16, 256>(o, plain, ep, st)
                        : launch_pair<Kind::F16, 128>(o, plain, ep, st);

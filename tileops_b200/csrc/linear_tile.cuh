@@ -235,10 +235,12 @@ inline int chunk_map(CUtensorMap* out, const void* p, int64_t rows, int64_t cols
                    CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-// Whether output or residual need the plain path: fp32, or rows that TMA cannot address.
+// Whether output or residual need the plain path: fp32, rows that TMA cannot address, or rows of C
+// that end inside 16 bytes: a TMA store writes those 16 bytes whole, the next columns of a wider
+// row with them.
 inline bool aligned_rows(const void* p, int64_t pitch);
-inline bool plain_output(const LinEpi& ep) {
-  return ep.dtype == TO_F32 || !aligned_rows(ep.c, ep.ldc * 2) ||
+inline bool plain_output(const LinEpi& ep, int64_t N) {
+  return ep.dtype == TO_F32 || N % 8 != 0 || !aligned_rows(ep.c, ep.ldc * 2) ||
          (ep.res != nullptr && !aligned_rows(ep.res, ep.ldr * 2));
 }
 inline bool aligned_rows(const void* p, int64_t pitch) {
