@@ -12,9 +12,10 @@
 // microsecond, and signals that cross SMs cost more than that. Wide tiles nearly halve the
 // operand bytes per product against 128 x 128 (44 KB per slice and 128 x 224 results).
 //
-// Bound by shared memory: a slice's 44 KB are written by the copies and read by the MMAs, 88 KB at
-// 128 B a clock, 700 clocks for MMAs of 450. 4096 x 7168 x 7168 FP8 with a residual: 242 us in a lone
-// launch, 1.74 PFLOP/s, and 283 us back to back (power cap); on CTA pairs it was 442 us.
+// 4096 x 7168 x 7168 FP8 with a residual: 237 to 246 us in a lone launch, 1.7 to 1.8 PFLOP/s, and 282
+// to 287 us back to back (power cap); on CTA pairs it was 442 us. That is some 1170 clocks a slice,
+// of which the MMAs need 450 and shared memory 700 (44 KB written by the copies, 44 KB read by the
+// MMAs, at 128 B a clock); where the other 470 go has not been measured.
 //
 // Every wait is bounded (kWaitLimitNs).
 #include <string.h>
@@ -82,7 +83,8 @@ __device__ __forceinline__ void tmem_ld_wait16(uint32_t* r) {
 }
 
 // OUT_ROWS: output or residual is no TMA tensor; a form of its own, since the other's registers are
-// all taken (with both in one, 7168 x 7168 at 4096 tokens took 358 us instead of 281).
+// all taken (with both in one, 7168 x 7168 at 4096 tokens took 358 us instead of 281). At 224 columns
+// it spills some 110 bytes a thread.
 template <Kind KD, int BN, bool OUT_ROWS>
 __global__ void __launch_bounds__(kThreadsB, 1)
     k_linear_bs(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,

@@ -14,9 +14,9 @@
 // chunks ahead of its use; results leave by TMA stores. (Turned by generic stores and written in
 // 16-byte pieces instead, 4096 x 512 -> 4096 FP8 with residual took 36 us instead of 28.)
 //
-// Bound by the tensor cores under the power cap: 2048 x 8192 x 28672 bf16 with bias and gelu 743 us,
-// 1.29 PFLOP/s (1.40 sustained by a plain library product); FP8 8192^3 with bias, gelu and residual
-// 438 us, 2.51 PFLOP/s. Between 65 and some 1000 tokens, by the operands through L2: 512 tokens of FP8
+// Bound by the tensor cores under the power cap: 2048 x 8192 x 28672 bf16 with bias and gelu 635 to
+// 820 us on different boxes and in longer or shorter runs, 1.17 to 1.51 PFLOP/s (a plain library
+// product: 1.40 sustained); FP8 8192^3 with bias, gelu and residual 370 to 476 us, 2.3 to 3.0. Between 65 and some 1000 tokens, by the operands through L2: 512 tokens of FP8
 // 7168 -> 2048 15 us, 128 tokens of bf16 1024 -> 28672 18 us.
 //
 // Roles: warp 0 copies of A, warp 1 MMA issue (leader CTA) and TMEM, warps 2..9 epilogue (two per
