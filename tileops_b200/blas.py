@@ -61,7 +61,8 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
     kernel, A (M, K), B (K, N), bias (N,), residual (M, N), all of one dtype (float32, float16 or
     bfloat16); ``act`` None, ``"relu"``, ``"silu"`` or ``"gelu"`` (tanh form, as in gelu_and_mul).
     The sum, the bias, the activation and the residual are fp32 and C is rounded once. Rows of A,
-    residual and out may be strided. ``out`` may be ``residual`` (added in place); it must not
+    residual and out may be strided; B is copied first unless it is row-major and dense. float32
+    operands run on SIMT tiles, 16-bit ones on the tensor cores. ``out`` may be ``residual`` (added in place); it must not
     overlap it otherwise, nor A, B or bias (ValueError)."""
     op = "gemm_bias_act"
     if a.ndim != 2 or b.ndim != 2:

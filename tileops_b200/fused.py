@@ -223,7 +223,8 @@ def add_rms_norm_group_quant(x: torch.Tensor, weight: torch.Tensor, group_size: 
     Returns ``(q, scales)``, or ``(q, scales, h)`` with a residual, h rounded to ``x.dtype``:
     written to ``residual_out`` when given, which may be ``x`` or ``residual`` itself. A row with
     a NaN has NaN scales, e4m3 NaN codes and int8 zeros; a row of zeros has codes 0 and scales
-    quant_eps / qmax (with ``eps`` 0 it is 0 / 0: NaN)."""
+    quant_eps / qmax (with ``eps`` 0 it is 0 / 0: NaN). The mean of squares is fp32: values beyond
+    about 1e19 overflow it, and their row's codes become 0."""
     op = "add_rms_norm_group_quant"
     if x.dim() == 0 or weight.shape != x.shape[-1:]:
         raise ValueError(f"{op}: weight.shape={tuple(weight.shape)} does not match the last "
